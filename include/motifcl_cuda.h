@@ -338,6 +338,54 @@ int mcl_cuda_gqa_backward(mcl_cuda_ctx* ctx, const float* q, const float* k, con
                           size_t batch, size_t query_tokens, size_t key_tokens, size_t n_head, size_t n_kv_head,
                           size_t head_dim, int causal, size_t query_offset, float scale);
 
+/* ---- layer norm (no reference counterpart on the Vulkan seam; next to rmsnorm above).
+ *   layernorm            out = (x - mean) / sqrt(var + eps) * weight + bias, mean and var of each row   x, out [rows, cols]; bias may be
+ *                        NULL; out may be x; row_stats [rows, 2] receives the mean and 1 / sqrt(var + eps) (NULL: not kept)
+ *   layernorm_backward   from the row_stats of the forward call: grad_x [rows, cols], grad_weight and grad_bias [cols] (overwritten, not
+ *                        added to); any of the three may be NULL.  grad_x may be grad_out or x itself.  Sums over the rows have a fixed
+ *                        order: the same call gives the same bits.  Takes workspace for partial sums, at most 8 MiB up to 4096 columns.
+ * ---- */
+int mcl_cuda_layernorm(mcl_cuda_ctx* ctx, const float* x, const float* weight, const float* bias, float* out, float* row_stats, size_t rows,
+                       size_t cols, float eps);
+int mcl_cuda_layernorm_backward(mcl_cuda_ctx* ctx, const float* x, const float* weight, const float* grad_out, const float* row_stats,
+                                float* grad_x, float* grad_weight, float* grad_bias, size_t rows, size_t cols);
+
+/* ---- what rows of logits say about tokens, and what they learn from a teacher's (no reference counterpart; next to softmax_cross_entropy
+ * above).  logits [rows, cols] with row_stride >= cols floats from row to row; columns behind cols are neither read nor written.  p = the
+ * softmax of a row's logits / temperature.
+ *   token_logprobs            logprobs [rows] = ln p of the row's token (0 for a token outside [0, cols): padding; tokens and logprobs may be
+ *                             NULL together); entropy [rows] (or NULL) = -sum p ln p; top_ids, top_logprobs [rows, n_top] (one of them may be
+ *                             NULL, both with n_top = 0): the n_top largest logits' places and ln p, largest first, equal ones by their
+ *                             place; row_stats [rows, 2] (or NULL) for the backward call: the largest logit m and s = sum exp((logit - m) /
+ *                             temperature), so that the logarithm of the softmax's denominator is m / temperature + ln s
+ *   ..._backward              grad_logits of sum(grad_logprobs . logprobs + grad_entropy . entropy); either gradient [rows] may be NULL (with it
+ *                             tokens or entropy)
+ *   distillation_loss         the Kullback-Leibler divergence of p from the teacher's kept tokens: t = softmax of the row's teacher_logits /
+ *                             temperature over its entries, partial [rows] = sum t (ln t - ln p[id]), out[0] = their mean over all rows.
+ *                             teacher_ids, teacher_logits [rows, n_teacher], logits or log probabilities (a constant per row falls out); an id
+ *                             outside [0, cols) is no entry, a row without entries has loss 0; an id named twice is two entries.  With
+ *                             grad_out and grad_logits (both or neither) also grad_logits = grad_out[0] * the gradient of out[0], in the same
+ *                             pass over the logits.  No factor temperature^2 is applied.
+ *   ..._backward              the same gradient from row_stats, for a grad_out that is known later
+ * grad_logits has the logits' stride, may be the logits themselves, and is exactly 0 in rows that nothing asks anything of (a token or ids
+ * outside the vocabulary and no other gradient, or gradients of 0), whatever these rows hold.
+ * Logits of -infinity (or the lowest float) are masked: p = 0, no part in the entropy, gradient 0.  A row of nothing but -infinity has
+ * logprobs and top_logprobs -infinity, entropy 0, an infinite distillation loss (0 without entries) and gradient 0.  A row with a NaN or +infinity gives NaN, and ids
+ * of -1.  Lists have at most MCL_CUDA_LIST_MAX tokens. ---- */
+#define MCL_CUDA_LIST_MAX 128
+int mcl_cuda_token_logprobs(mcl_cuda_ctx* ctx, const float* logits, const int32_t* tokens, float* logprobs, float* entropy, int32_t* top_ids,
+                            float* top_logprobs, float* row_stats, size_t rows, size_t cols, size_t row_stride, size_t n_top,
+                            float temperature);
+int mcl_cuda_token_logprobs_backward(mcl_cuda_ctx* ctx, const float* logits, const int32_t* tokens, const float* row_stats, const float* entropy,
+                                     const float* grad_logprobs, const float* grad_entropy, float* grad_logits, size_t rows, size_t cols,
+                                     size_t row_stride, float temperature);
+int mcl_cuda_distillation_loss(mcl_cuda_ctx* ctx, const float* logits, const int32_t* teacher_ids, const float* teacher_logits, float* partial,
+                               float* out, float* row_stats, const float* grad_out, float* grad_logits, size_t rows, size_t cols,
+                               size_t row_stride, size_t n_teacher, float temperature);
+int mcl_cuda_distillation_loss_backward(mcl_cuda_ctx* ctx, const float* logits, const int32_t* teacher_ids, const float* teacher_logits,
+                                        const float* row_stats, const float* grad_out, float* grad_logits, size_t rows, size_t cols,
+                                        size_t row_stride, size_t n_teacher, float temperature);
+
 /* ---- the remaining fp32 ops of the ternary15m trainer step (tools/train_ternary15m.cpp:273-293,377): they replace
  * run_vulkan_token_position_embedding (:821), run_vulkan_embedding_gather (:776), run_vulkan_embedding_weight_backward
  * and its _scatter / _scatter_cas variants (:784-819), run_vulkan_position_embedding_backward (:832), run_vulkan_rope /

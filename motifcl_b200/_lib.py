@@ -99,6 +99,12 @@ def lib() -> C.CDLL:
         L.mcl_cuda_rmsnorm.argtypes = [vp, vp, vp, vp, sz, sz, f]
         L.mcl_cuda_rmsnorm_backward_x.argtypes = [vp, vp, vp, vp, vp, sz, sz, f]
         L.mcl_cuda_rmsnorm_backward_weight.argtypes = [vp, vp, vp, vp, vp, sz, sz, f]
+        L.mcl_cuda_layernorm.argtypes = [vp, vp, vp, vp, vp, vp, sz, sz, f]
+        L.mcl_cuda_layernorm_backward.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, sz, sz]
+        L.mcl_cuda_token_logprobs.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, sz, sz, sz, sz, f]
+        L.mcl_cuda_token_logprobs_backward.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, sz, sz, sz, f]
+        L.mcl_cuda_distillation_loss.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, sz, sz, sz, f]
+        L.mcl_cuda_distillation_loss_backward.argtypes = [vp, vp, vp, vp, vp, vp, vp, sz, sz, sz, sz, f]
         L.mcl_cuda_swiglu.argtypes = [vp, vp, vp, sz, sz]
         L.mcl_cuda_mse_loss_partial.argtypes = [vp, vp, vp, vp, sz]
         L.mcl_cuda_peer_allreduce_f32.argtypes = [vp, C.POINTER(vp), C.POINTER(vp), C.c_int, C.c_int, sz, sz, C.c_int, vp]

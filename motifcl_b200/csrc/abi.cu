@@ -1294,6 +1294,42 @@ int mcl_cuda_rmsnorm_backward_weight(mcl_cuda_ctx* ctx, const float* x, const fl
     if (cols > 1024) ctx->launches += 1;     // a row pass and a column pass
     return MCL_CUDA_OK;
 }
+int mcl_cuda_layernorm(mcl_cuda_ctx* ctx, const float* x, const float* weight, const float* bias, float* out, float* row_stats, size_t rows,
+                       size_t cols, float eps) {
+    MCL_NEED_CTX(ctx);
+    const char* op = "layernorm";
+    MCL_TRY(check_rows(ctx, op, rows, cols));
+    if (!std::isfinite(eps) || eps < 0.0f) return fail(ctx, MCL_CUDA_EINVAL, "layernorm requires non-negative finite eps");
+    MCL_TRY(check_ptr(ctx, op, "x", x, 4));
+    MCL_TRY(check_ptr(ctx, op, "weight", weight, 4));
+    if (bias) MCL_TRY(check_ptr(ctx, op, "bias", bias, 4));
+    MCL_TRY(check_ptr(ctx, op, "out", out, 4));
+    if (row_stats) MCL_TRY(check_ptr(ctx, op, "row_stats", row_stats, 4));
+    DeviceGuard guard(ctx->device);
+    MCL_LAUNCH(ctx, op, mcl::launch_layernorm(x, weight, bias, out, row_stats, rows, (int)cols, eps, ctx->sm_count, ctx->stream));
+    return MCL_CUDA_OK;
+}
+int mcl_cuda_layernorm_backward(mcl_cuda_ctx* ctx, const float* x, const float* weight, const float* grad_out, const float* row_stats,
+                                float* grad_x, float* grad_weight, float* grad_bias, size_t rows, size_t cols) {
+    MCL_NEED_CTX(ctx);
+    const char* op = "layernorm backward";
+    MCL_TRY(check_rows(ctx, op, rows, cols));
+    MCL_TRY(check_ptr(ctx, op, "x", x, 4));
+    MCL_TRY(check_ptr(ctx, op, "weight", weight, 4));
+    MCL_TRY(check_ptr(ctx, op, "grad_out", grad_out, 4));
+    MCL_TRY(check_ptr(ctx, op, "row_stats", row_stats, 4));
+    if (!grad_x && !grad_weight && !grad_bias) return fail(ctx, MCL_CUDA_EINVAL, "layernorm backward: no output is asked for");
+    if (grad_x) MCL_TRY(check_ptr(ctx, op, "grad_x", grad_x, 4));
+    if (grad_weight) MCL_TRY(check_ptr(ctx, op, "grad_weight", grad_weight, 4));
+    if (grad_bias) MCL_TRY(check_ptr(ctx, op, "grad_bias", grad_bias, 4));
+    DeviceGuard guard(ctx->device);
+    void* ws = nullptr;
+    const size_t floats = mcl::layernorm_partial_floats(rows, (int)cols, grad_weight != nullptr, grad_bias != nullptr, ctx->sm_count);
+    if (floats) MCL_TRY(ws_reserve(ctx, floats * sizeof(float), &ws));
+    MCL_TC(ctx, op, mcl::launch_layernorm_backward(x, weight, grad_out, row_stats, grad_x, grad_weight, grad_bias, static_cast<float*>(ws), rows,
+                                                   (int)cols, ctx->sm_count, ctx->stream, &_n));
+    return MCL_CUDA_OK;
+}
 int mcl_cuda_mse_loss_partial(mcl_cuda_ctx* ctx, const float* pred, const float* target, float* partial, size_t n) {
     MCL_NEED_CTX(ctx);
     const char* op = "mse_loss_partial";
@@ -1375,6 +1411,116 @@ int mcl_cuda_softmax_cross_entropy_backward(mcl_cuda_ctx* ctx, const float* logi
     MCL_TRY(check_ptr(ctx, op, "grad_logits", grad_logits, 4));
     DeviceGuard guard(ctx->device);
     MCL_LAUNCH(ctx, op, mcl::launch_softmax_cross_entropy_backward(logits, targets, grad_out, grad_logits, rows, (int)cols, ctx->sm_count, ctx->stream));
+    return MCL_CUDA_OK;
+}
+
+// ---- rows of logits: what they say about tokens, and what they learn from a teacher's ---------------------
+namespace {
+int check_vocab(mcl_cuda_ctx* ctx, const char* op, const float* logits, size_t rows, size_t cols, size_t row_stride, float temperature) {
+    MCL_TRY(check_rows(ctx, op, rows, cols));
+    if (row_stride < cols) return fail(ctx, MCL_CUDA_EINVAL, std::string(op) + " requires row_stride >= cols");
+    if (row_stride > (size_t)-1 / sizeof(float) / rows) return fail(ctx, MCL_CUDA_EINVAL, std::string(op) + " dimension is too large");
+    if (!(temperature > 0.0f) || !std::isfinite(temperature) || !(1.0f / temperature >= 1e-30f) || !(1.0f / temperature <= 1e30f))
+        return fail(ctx, MCL_CUDA_EINVAL, std::string(op) + " requires a temperature from 1e-30 to 1e30");
+    return check_ptr(ctx, op, "logits", logits, 4);
+}
+// grad_logits may be the logits themselves, and overlap them in no other way
+int check_grad_logits(mcl_cuda_ctx* ctx, const char* op, const float* logits, const float* grad_logits, size_t rows, size_t cols, size_t row_stride) {
+    MCL_TRY(check_ptr(ctx, op, "grad_logits", grad_logits, 4));
+    const uintptr_t a = reinterpret_cast<uintptr_t>(logits), b = reinterpret_cast<uintptr_t>(grad_logits);
+    const size_t span = ((rows - 1) * row_stride + cols) * sizeof(float);
+    if (a != b && a < b + span && b < a + span)
+        return fail(ctx, MCL_CUDA_EINVAL, std::string(op) + ": grad_logits overlaps logits without being the same");
+    return MCL_CUDA_OK;
+}
+int check_teacher(mcl_cuda_ctx* ctx, const char* op, const int32_t* teacher_ids, const float* teacher_logits, size_t n_teacher) {
+    if (n_teacher == 0 || n_teacher > MCL_CUDA_LIST_MAX)
+        return fail(ctx, MCL_CUDA_EINVAL, std::string(op) + " requires 1 to " + std::to_string(MCL_CUDA_LIST_MAX) + " teacher tokens per row");
+    MCL_TRY(check_ptr(ctx, op, "teacher_ids", teacher_ids, 4));
+    return check_ptr(ctx, op, "teacher_logits", teacher_logits, 4);
+}
+static_assert(MCL_CUDA_LIST_MAX == mcl::kVocabListMax, "the longest list of the header is the kernels'");
+}  // namespace
+
+int mcl_cuda_token_logprobs(mcl_cuda_ctx* ctx, const float* logits, const int32_t* tokens, float* logprobs, float* entropy, int32_t* top_ids,
+                            float* top_logprobs, float* row_stats, size_t rows, size_t cols, size_t row_stride, size_t n_top,
+                            float temperature) {
+    MCL_NEED_CTX(ctx);
+    const char* op = "token_logprobs";
+    MCL_TRY(check_vocab(ctx, op, logits, rows, cols, row_stride, temperature));
+    if (n_top > MCL_CUDA_LIST_MAX || n_top > cols)
+        return fail(ctx, MCL_CUDA_EINVAL, "token_logprobs: n_top exceeds " + std::to_string(MCL_CUDA_LIST_MAX) + " or cols");
+    if ((tokens == nullptr) != (logprobs == nullptr)) return fail(ctx, MCL_CUDA_EINVAL, "token_logprobs: tokens and logprobs go together");
+    if ((n_top == 0) != (top_ids == nullptr && top_logprobs == nullptr))
+        return fail(ctx, MCL_CUDA_EINVAL, "token_logprobs: n_top and its outputs go together");
+    if (!logprobs && !entropy && !row_stats && n_top == 0) return fail(ctx, MCL_CUDA_EINVAL, "token_logprobs: no output is asked for");
+    if (tokens) MCL_TRY(check_ptr(ctx, op, "tokens", tokens, 4));
+    if (logprobs) MCL_TRY(check_ptr(ctx, op, "logprobs", logprobs, 4));
+    if (entropy) MCL_TRY(check_ptr(ctx, op, "entropy", entropy, 4));
+    if (top_ids) MCL_TRY(check_ptr(ctx, op, "top_ids", top_ids, 4));
+    if (top_logprobs) MCL_TRY(check_ptr(ctx, op, "top_logprobs", top_logprobs, 4));
+    if (row_stats) MCL_TRY(check_ptr(ctx, op, "row_stats", row_stats, 4));
+    DeviceGuard guard(ctx->device);
+    MCL_LAUNCH(ctx, op, mcl::launch_token_logprobs(logits, tokens, logprobs, entropy, top_ids, top_logprobs, row_stats, rows, (int)cols, row_stride,
+                                                   (int)n_top, temperature, ctx->sm_count, ctx->stream));
+    return MCL_CUDA_OK;
+}
+int mcl_cuda_token_logprobs_backward(mcl_cuda_ctx* ctx, const float* logits, const int32_t* tokens, const float* row_stats, const float* entropy,
+                                     const float* grad_logprobs, const float* grad_entropy, float* grad_logits, size_t rows, size_t cols,
+                                     size_t row_stride, float temperature) {
+    MCL_NEED_CTX(ctx);
+    const char* op = "token_logprobs backward";
+    MCL_TRY(check_vocab(ctx, op, logits, rows, cols, row_stride, temperature));
+    MCL_TRY(check_ptr(ctx, op, "row_stats", row_stats, 4));
+    if (!grad_logprobs && !grad_entropy) return fail(ctx, MCL_CUDA_EINVAL, "token_logprobs backward: no gradient is given");
+    if (grad_logprobs) {
+        MCL_TRY(check_ptr(ctx, op, "grad_logprobs", grad_logprobs, 4));
+        MCL_TRY(check_ptr(ctx, op, "tokens", tokens, 4));
+    }
+    if (grad_entropy) {
+        MCL_TRY(check_ptr(ctx, op, "grad_entropy", grad_entropy, 4));
+        MCL_TRY(check_ptr(ctx, op, "entropy", entropy, 4));
+    }
+    MCL_TRY(check_grad_logits(ctx, op, logits, grad_logits, rows, cols, row_stride));
+    DeviceGuard guard(ctx->device);
+    MCL_LAUNCH(ctx, op, mcl::launch_token_logprobs_backward(logits, tokens, row_stats, entropy, grad_logprobs, grad_entropy, grad_logits, rows, (int)cols,
+                                                            row_stride, temperature, ctx->sm_count, ctx->stream));
+    return MCL_CUDA_OK;
+}
+int mcl_cuda_distillation_loss(mcl_cuda_ctx* ctx, const float* logits, const int32_t* teacher_ids, const float* teacher_logits, float* partial,
+                               float* out, float* row_stats, const float* grad_out, float* grad_logits, size_t rows, size_t cols,
+                               size_t row_stride, size_t n_teacher, float temperature) {
+    MCL_NEED_CTX(ctx);
+    const char* op = "distillation_loss";
+    MCL_TRY(check_vocab(ctx, op, logits, rows, cols, row_stride, temperature));
+    MCL_TRY(check_teacher(ctx, op, teacher_ids, teacher_logits, n_teacher));
+    MCL_TRY(check_ptr(ctx, op, "partial", partial, 4));
+    MCL_TRY(check_ptr(ctx, op, "out", out, 4));
+    if (row_stats) MCL_TRY(check_ptr(ctx, op, "row_stats", row_stats, 4));
+    if ((grad_out == nullptr) != (grad_logits == nullptr)) return fail(ctx, MCL_CUDA_EINVAL, "distillation_loss: grad_out and grad_logits go together");
+    if (grad_logits) {
+        MCL_TRY(check_ptr(ctx, op, "grad_out", grad_out, 4));
+        MCL_TRY(check_grad_logits(ctx, op, logits, grad_logits, rows, cols, row_stride));
+    }
+    DeviceGuard guard(ctx->device);
+    MCL_LAUNCH(ctx, op, mcl::launch_distillation_loss(logits, teacher_ids, teacher_logits, partial, out, row_stats, grad_out, grad_logits, rows, (int)cols,
+                                                      row_stride, (int)n_teacher, temperature, ctx->sm_count, ctx->stream));
+    ctx->launches += 1;     // row losses, then their mean
+    return MCL_CUDA_OK;
+}
+int mcl_cuda_distillation_loss_backward(mcl_cuda_ctx* ctx, const float* logits, const int32_t* teacher_ids, const float* teacher_logits,
+                                        const float* row_stats, const float* grad_out, float* grad_logits, size_t rows, size_t cols,
+                                        size_t row_stride, size_t n_teacher, float temperature) {
+    MCL_NEED_CTX(ctx);
+    const char* op = "distillation_loss backward";
+    MCL_TRY(check_vocab(ctx, op, logits, rows, cols, row_stride, temperature));
+    MCL_TRY(check_teacher(ctx, op, teacher_ids, teacher_logits, n_teacher));
+    MCL_TRY(check_ptr(ctx, op, "row_stats", row_stats, 4));
+    MCL_TRY(check_ptr(ctx, op, "grad_out", grad_out, 4));
+    MCL_TRY(check_grad_logits(ctx, op, logits, grad_logits, rows, cols, row_stride));
+    DeviceGuard guard(ctx->device);
+    MCL_LAUNCH(ctx, op, mcl::launch_distillation_loss_backward(logits, teacher_ids, teacher_logits, row_stats, grad_out, grad_logits, rows, (int)cols,
+                                                               row_stride, (int)n_teacher, temperature, ctx->sm_count, ctx->stream));
     return MCL_CUDA_OK;
 }
 

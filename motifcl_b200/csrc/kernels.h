@@ -260,6 +260,14 @@ cudaError_t launch_rope(const float* x, float* out, size_t rows, int tokens, int
                         cudaStream_t stream);
 cudaError_t launch_adam(float* param, const float* grad, float* m, float* v, size_t n, float lr, float beta1, float beta2,
                         float eps, float weight_decay, float c1, float c2, int sm_count, cudaStream_t stream);
+cudaError_t launch_mean(const float* in, float* out, size_t n, size_t denominator, cudaStream_t stream);
+// weight [cols], bias [cols] or null; row_stats [rows][2] (or null): mean and inverse deviation
+cudaError_t launch_layernorm(const float* x, const float* w, const float* b, float* out, float* row_stats, size_t rows, int cols, float eps,
+                             int sm_count, cudaStream_t stream);
+// partial: layernorm_partial_floats() floats of scratch; dx, dw, db may be null
+size_t layernorm_partial_floats(size_t rows, int cols, bool dw, bool db, int sm_count);
+cudaError_t launch_layernorm_backward(const float* x, const float* w, const float* dy, const float* row_stats, float* dx, float* dw, float* db,
+                                      float* partial, size_t rows, int cols, int sm_count, cudaStream_t stream, int* launches);
 size_t gqa_forward_scratch_floats(int batch, int tq, int tk, int n_head, int hd, int vhd);
 cudaError_t launch_gqa_forward(const float* q, const float* k, const float* v, float* out, int batch, int tq, int tk,
                                int key_stride, int n_head, int n_kv, int hd, int vhd, int causal, int q_off, int window,
@@ -267,5 +275,21 @@ cudaError_t launch_gqa_forward(const float* q, const float* k, const float* v, f
 cudaError_t launch_gqa_backward(const float* q, const float* k, const float* v, const float* dout, float* probs, float* ds,
                                 float* dq, float* dk, float* dv, int batch, int tq, int tk, int n_head, int n_kv, int hd,
                                 int causal, int q_off, float scale, cudaStream_t stream, int* launches);
+
+// vocab_rows.cu -- what rows of logits say about tokens, and what they learn from a teacher's (row_stats [rows][2]: largest logit, sum of
+// exponentials)
+constexpr int kVocabListMax = 128;     // tokens of a row's list
+cudaError_t launch_token_logprobs(const float* logits, const int* tokens, float* logprobs, float* entropy, int* top_ids, float* top_logprobs,
+                                  float* row_stats, size_t rows, int cols, size_t stride, int n_top, float temperature, int sm_count,
+                                  cudaStream_t stream);
+cudaError_t launch_token_logprobs_backward(const float* logits, const int* tokens, const float* row_stats, const float* entropy,
+                                           const float* grad_logprobs, const float* grad_entropy, float* grad_logits, size_t rows, int cols,
+                                           size_t stride, float temperature, int sm_count, cudaStream_t stream);
+cudaError_t launch_distillation_loss(const float* logits, const int* teacher_ids, const float* teacher_logits, float* losses, float* out,
+                                     float* row_stats, const float* grad_out, float* grad_logits, size_t rows, int cols, size_t stride,
+                                     int n_teacher, float temperature, int sm_count, cudaStream_t stream);
+cudaError_t launch_distillation_loss_backward(const float* logits, const int* teacher_ids, const float* teacher_logits, const float* row_stats,
+                                              const float* grad_out, float* grad_logits, size_t rows, int cols, size_t stride, int n_teacher,
+                                              float temperature, int sm_count, cudaStream_t stream);
 
 }  // namespace mcl

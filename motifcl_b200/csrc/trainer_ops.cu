@@ -212,6 +212,113 @@ __global__ void __launch_bounds__(256) rmsnorm_bwd_w_kernel(const float* x, cons
     }
 }
 
+// ---- layer norm --------------------------------------------------------------------------------
+// y = (x - mean) r w + b with r = 1 / sqrt(var + eps).  With n = (x - mean) r and g = dy w:
+//     dx = r (g - mean(g) - n mean(g n))      dw = sum of dy n over the rows      db = sum of dy
+// The variance is the mean of (x - mean)^2, not a difference of two sums, which a mean far from zero would leave no digits of.
+// A block per row; rows are read again from L1.
+__global__ void __launch_bounds__(256) layernorm_kernel(const float* x, const float* w, const float* b, float* out, float* row_stats, size_t rows,
+                                                        Vec4 a, float eps) {
+    grid_release();
+    grid_wait();
+    __shared__ float red[32];
+    for (size_t row = blockIdx.x; row < rows; row += gridDim.x) {
+        const float* xr = x + row * (size_t)a.cols;
+        float sum = 0.0f, sq = 0.0f;
+        for (int c = 4 * threadIdx.x; c < a.cols; c += 1024) { const float4 v = a.get(xr, c); sum += (v.x + v.y) + (v.z + v.w); }
+        const float mean = block_sum(sum, red) / (float)a.cols;
+        for (int c = 4 * threadIdx.x; c < a.cols; c += 1024) {
+            const float4 v = a.get(xr, c);
+            const float d0 = v.x - mean, d1 = c + 1 < a.cols ? v.y - mean : 0.0f, d2 = c + 2 < a.cols ? v.z - mean : 0.0f, d3 = c + 3 < a.cols ? v.w - mean : 0.0f;
+            sq += (d0 * d0 + d1 * d1) + (d2 * d2 + d3 * d3);
+        }
+        const float inv = 1.0f / sqrtf(block_sum(sq, red) / (float)a.cols + eps);
+        float* o = out + row * (size_t)a.cols;
+        for (int c = 4 * threadIdx.x; c < a.cols; c += 1024) {
+            const float4 v = a.get(xr, c), wv = a.get(w, c), bv = b != nullptr ? a.get(b, c) : make_float4(0.f, 0.f, 0.f, 0.f);
+            a.put(o, c, make_float4((v.x - mean) * inv * wv.x + bv.x, (v.y - mean) * inv * wv.y + bv.y, (v.z - mean) * inv * wv.z + bv.z,
+                                    (v.w - mean) * inv * wv.w + bv.w));
+        }
+        if (row_stats != nullptr && threadIdx.x == 0) { row_stats[2 * row] = mean; row_stats[2 * row + 1] = inv; }
+    }
+}
+__global__ void __launch_bounds__(256) layernorm_bwd_x_kernel(const float* x, const float* w, const float* dy, const float* row_stats, float* dx,
+                                                              size_t rows, Vec4 a) {
+    grid_release();
+    grid_wait();
+    __shared__ float red[32];
+    for (size_t row = blockIdx.x; row < rows; row += gridDim.x) {
+        const float* xr = x + row * (size_t)a.cols;
+        const float* gr = dy + row * (size_t)a.cols;
+        const float mean = row_stats[2 * row], inv = row_stats[2 * row + 1];
+        float sg = 0.0f, sgn = 0.0f;
+        for (int c = 4 * threadIdx.x; c < a.cols; c += 1024) {          // columns behind the row read as g = 0
+            const float4 v = a.get(xr, c), gv = a.get(gr, c), wv = a.get(w, c);
+            const float4 g = make_float4(gv.x * wv.x, gv.y * wv.y, gv.z * wv.z, gv.w * wv.w);
+            sg += (g.x + g.y) + (g.z + g.w);
+            sgn += dot4(g, make_float4((v.x - mean) * inv, (v.y - mean) * inv, (v.z - mean) * inv, (v.w - mean) * inv));
+        }
+        sg = block_sum(sg, red) / (float)a.cols;
+        sgn = block_sum(sgn, red) / (float)a.cols;
+        float* o = dx + row * (size_t)a.cols;
+        auto one = [&](float v, float g) { return inv * (g - sg - (v - mean) * inv * sgn); };
+        for (int c = 4 * threadIdx.x; c < a.cols; c += 1024) {
+            const float4 v = a.get(xr, c), gv = a.get(gr, c), wv = a.get(w, c);
+            a.put(o, c, make_float4(one(v.x, gv.x * wv.x), one(v.y, gv.y * wv.y), one(v.z, gv.z * wv.z), one(v.w, gv.w * wv.w)));
+        }
+    }
+}
+// partial sums of dw (and db) over the rows of a split; blockIdx.y = split
+__global__ void __launch_bounds__(256) layernorm_bwd_w_kernel(const float* x, const float* dy, const float* row_stats, float* dw_part, float* db_part,
+                                                              size_t rows, int cols, size_t rows_per_split) {
+    grid_release();
+    grid_wait();
+    __shared__ float part[2][8][33];
+    const int cx = threadIdx.x & 31, ry = threadIdx.x >> 5;
+    const int col = blockIdx.x * 32 + cx;
+    const size_t r0 = (size_t)blockIdx.y * rows_per_split;
+    const size_t r1 = r0 + rows_per_split < rows ? r0 + rows_per_split : rows;
+    float aw = 0.0f, ab = 0.0f;
+    if (col < cols)
+        for (size_t r = r0 + ry; r < r1; r += 8) {
+            const float g = dy[r * cols + col];
+            aw += g * ((x[r * cols + col] - row_stats[2 * r]) * row_stats[2 * r + 1]);
+            ab += g;
+        }
+    part[0][ry][cx] = aw;
+    part[1][ry][cx] = ab;
+    __syncthreads();
+    if (ry < 2 && col < cols) {
+        float s = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s += part[ry][j][cx];
+        float* to = ry == 0 ? dw_part : db_part;
+        if (to != nullptr) to[(size_t)blockIdx.y * cols + col] = s;
+    }
+}
+// out[c] = sum of part[i][c] over the splits, always in the same order; blockIdx.y: weight, bias
+__global__ void __launch_bounds__(256) layernorm_sum_kernel(const float* dw_part, const float* db_part, float* dw, float* db, int splits, int cols) {
+    grid_release();
+    grid_wait();
+    __shared__ float part[8][33];
+    const int cx = threadIdx.x & 31, ry = threadIdx.x >> 5;
+    const int col = blockIdx.x * 32 + cx;
+    const float* from = blockIdx.y == 0 ? dw_part : db_part;
+    float* to = blockIdx.y == 0 ? dw : db;
+    if (to == nullptr) return;
+    float s = 0.0f;
+    if (col < cols)
+        for (int i = ry; i < splits; i += 8) s += from[(size_t)i * cols + col];
+    part[ry][cx] = s;
+    __syncthreads();
+    if (ry == 0 && col < cols) {
+        s = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s += part[j][cx];
+        to[col] = s;
+    }
+}
+
 // ---- swiglu ----------------------------------------------------------------------------------
 // W = 4: 128-bit accesses (hidden % 4 == 0, 16-byte aligned tensors); HBM-bound, 4096 x 768: 14 us with scalar accesses.
 __device__ __forceinline__ void swiglu_grads(float gate, float up, float go, float& dg, float& du) {
@@ -715,6 +822,44 @@ cudaError_t launch_rmsnorm_backward_weight(const float* x, const float* dy, floa
     const size_t rows_per_block = (rows + splits - 1) / splits;
     launch_chained(rmsnorm_bwd_w_kernel, dim3(col_blocks, (unsigned)splits), dim3(256), 0, stream, x, dy, row_inv, dw, rows, cols, rows_per_block);
     return cudaGetLastError();
+}
+cudaError_t launch_layernorm(const float* x, const float* w, const float* b, float* out, float* row_stats, size_t rows, int cols, float eps,
+                             int sm_count, cudaStream_t stream) {
+    const Vec4 a = {cols % 4 == 0 && all16(x, w, out, b), cols};
+    launch_chained(layernorm_kernel, dim3(row_grid(rows, sm_count)), dim3(256), 0, stream, x, w, b, out, row_stats, rows, a, eps);
+    return cudaGetLastError();
+}
+namespace {
+size_t layernorm_splits(size_t rows, int cols, int sm_count) {
+    const size_t col_blocks = ((size_t)cols + 31) / 32;
+    size_t splits = ((size_t)sm_count * 8 + col_blocks - 1) / col_blocks;
+    if (splits > (rows + 63) / 64) splits = (rows + 63) / 64;
+    const size_t per = (rows + splits - 1) / splits;
+    return (rows + per - 1) / per;
+}
+}  // namespace
+size_t layernorm_partial_floats(size_t rows, int cols, bool dw, bool db, int sm_count) {
+    return (size_t)(dw + db) * layernorm_splits(rows, cols, sm_count) * (size_t)cols;
+}
+cudaError_t launch_layernorm_backward(const float* x, const float* w, const float* dy, const float* row_stats, float* dx, float* dw, float* db,
+                                      float* partial, size_t rows, int cols, int sm_count, cudaStream_t stream, int* launches) {
+    cudaError_t e;
+    if (dw != nullptr || db != nullptr) {           // first: dx may take the place of x or dy
+        const size_t splits = layernorm_splits(rows, cols, sm_count), per = (rows + splits - 1) / splits;
+        float* dw_part = dw != nullptr ? partial : nullptr;
+        float* db_part = db != nullptr ? partial + (dw != nullptr ? splits * (size_t)cols : 0) : nullptr;
+        const unsigned blocks = (unsigned)((cols + 31) / 32);
+        if ((e = launch_chained(layernorm_bwd_w_kernel, dim3(blocks, (unsigned)splits), dim3(256), 0, stream, x, dy, row_stats, dw_part, db_part, rows, cols, per)) != cudaSuccess) return e;
+        if ((e = launch_chained(layernorm_sum_kernel, dim3(blocks, 2), dim3(256), 0, stream, dw_part, db_part, dw, db, (int)splits, cols)) != cudaSuccess) return e;
+        *launches += 2;
+    }
+    if (dx == nullptr) return cudaSuccess;
+    const Vec4 a = {cols % 4 == 0 && all16(x, w, dy, dx), cols};
+    *launches += 1;
+    return launch_chained(layernorm_bwd_x_kernel, dim3(row_grid(rows, sm_count)), dim3(256), 0, stream, x, w, dy, row_stats, dx, rows, a);
+}
+cudaError_t launch_mean(const float* in, float* out, size_t n, size_t denominator, cudaStream_t stream) {
+    return launch_chained(mean_kernel, dim3(1), dim3(1024), 0, stream, in, out, n, denominator);
 }
 cudaError_t launch_swiglu(const float* packed, float* out, size_t rows, int hidden, int sm_count, cudaStream_t stream) {
     const size_t n = rows * (size_t)hidden;

@@ -228,6 +228,15 @@ class Context:
         self._check(self._lib.mcl_cuda_rmsnorm_backward_weight(self._ctx, _ptr(x), _ptr(grad_out), _ptr(row_inv),
                                                                _ptr(grad_weight), rows, cols, eps))
 
+    def layernorm(self, x, weight, bias, out, row_stats, rows, cols, eps):
+        """bias and row_stats (mean and inverse deviation of each row, for the backward call) may be None."""
+        self._check(self._lib.mcl_cuda_layernorm(self._ctx, _ptr(x), _ptr(weight), _ptr(bias), _ptr(out), _ptr(row_stats), rows, cols, eps))
+
+    def layernorm_backward(self, x, weight, grad_out, row_stats, grad_x, grad_weight, grad_bias, rows, cols):
+        """Any of the three gradients may be None."""
+        self._check(self._lib.mcl_cuda_layernorm_backward(self._ctx, _ptr(x), _ptr(weight), _ptr(grad_out), _ptr(row_stats), _ptr(grad_x),
+                                                          _ptr(grad_weight), _ptr(grad_bias), rows, cols))
+
     def mse_loss(self, pred, target, partial, out, n):
         """mean((pred - target)^2) with MotifCL's OpenCL summation order; partial: ceil(n / 256) floats."""
         self._check(self._lib.mcl_cuda_mse_loss_partial(self._ctx, _ptr(pred), _ptr(target), _ptr(partial), n))
@@ -250,6 +259,34 @@ class Context:
     def softmax_cross_entropy_backward(self, logits, targets, grad_out, grad_logits, rows, cols):
         self._check(self._lib.mcl_cuda_softmax_cross_entropy_backward(self._ctx, _ptr(logits), _ptr(targets),
                                                                       _ptr(grad_out), _ptr(grad_logits), rows, cols))
+
+    # ---- rows of logits (row_stride floats apart, default cols): what they say about tokens, and what they learn from a teacher's ----
+    def token_logprobs(self, logits, tokens, logprobs, entropy, top_ids, top_logprobs, row_stats, rows, cols, n_top=0, temperature=1.0,
+                       row_stride=None):
+        """ln p of each row's token, the row's entropy and its n_top most probable tokens; outputs that are None are not formed."""
+        self._check(self._lib.mcl_cuda_token_logprobs(
+            self._ctx, _ptr(logits), _ptr(tokens), _ptr(logprobs), _ptr(entropy), _ptr(top_ids), _ptr(top_logprobs), _ptr(row_stats), rows, cols,
+            cols if row_stride is None else row_stride, n_top, temperature))
+
+    def token_logprobs_backward(self, logits, tokens, row_stats, entropy, grad_logprobs, grad_entropy, grad_logits, rows, cols, temperature=1.0,
+                                row_stride=None):
+        """Gradient of the logits from those of logprobs and entropy (either may be None)."""
+        self._check(self._lib.mcl_cuda_token_logprobs_backward(
+            self._ctx, _ptr(logits), _ptr(tokens), _ptr(row_stats), _ptr(entropy), _ptr(grad_logprobs), _ptr(grad_entropy), _ptr(grad_logits), rows,
+            cols, cols if row_stride is None else row_stride, temperature))
+
+    def distillation_loss(self, logits, teacher_ids, teacher_logits, partial, out, row_stats, grad_out, grad_logits, rows, cols, n_teacher,
+                          temperature=1.0, row_stride=None):
+        """Loss against a teacher's kept tokens; with grad_out and grad_logits its gradient in the same pass."""
+        self._check(self._lib.mcl_cuda_distillation_loss(
+            self._ctx, _ptr(logits), _ptr(teacher_ids), _ptr(teacher_logits), _ptr(partial), _ptr(out), _ptr(row_stats), _ptr(grad_out),
+            _ptr(grad_logits), rows, cols, cols if row_stride is None else row_stride, n_teacher, temperature))
+
+    def distillation_loss_backward(self, logits, teacher_ids, teacher_logits, row_stats, grad_out, grad_logits, rows, cols, n_teacher,
+                                   temperature=1.0, row_stride=None):
+        self._check(self._lib.mcl_cuda_distillation_loss_backward(
+            self._ctx, _ptr(logits), _ptr(teacher_ids), _ptr(teacher_logits), _ptr(row_stats), _ptr(grad_out), _ptr(grad_logits), rows, cols,
+            cols if row_stride is None else row_stride, n_teacher, temperature))
 
     def token_position_embedding(self, token_weight, pos_weight, token_ids, out, token_count, vocab, seq_len, dim):
         self._check(self._lib.mcl_cuda_token_position_embedding(
