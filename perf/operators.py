@@ -84,8 +84,11 @@ def _logits(g, rows, vocab, pad, rounded=False, masked=0.0):
 
 
 def _context():
-    from motifcl_b200 import Context
-    return Context.on_torch_stream(torch.cuda.current_device())
+    """A program has one context for its stream, whatever inputs it meets."""
+    if not hasattr(_context, "kept"):
+        from motifcl_b200 import Context
+        _context.kept = Context.on_torch_stream(torch.cuda.current_device())
+    return _context.kept
 
 
 def prepare(case, seed):
