@@ -261,6 +261,7 @@ int check_device_error(mcl_cuda_ctx* ctx) {
             case 16: case 17: who = "work items (the drawing warp and its readers lost step)"; break;
             case 21: who = "wide-row counter update (a row slot was never marked ready or released)"; break;
             case 41: who = "single-layer kernel (a k-tile's MMAs never completed)"; break;
+            case 61: who = "distillation of long rows (a chunk of a row never arrived or was never done)"; break;
             case 31: who = "peer all-reduce (a rank never announced its partial result)"; break;
             default: who = "epilogue (accumulator never completed)"; break;
         }
@@ -1504,7 +1505,7 @@ int mcl_cuda_distillation_loss(mcl_cuda_ctx* ctx, const float* logits, const int
     }
     DeviceGuard guard(ctx->device);
     MCL_LAUNCH(ctx, op, mcl::launch_distillation_loss(logits, teacher_ids, teacher_logits, partial, out, row_stats, grad_out, grad_logits, rows, (int)cols,
-                                                      row_stride, (int)n_teacher, temperature, ctx->sm_count, ctx->stream));
+                                                      row_stride, (int)n_teacher, temperature, ctx->err_word, ctx->sm_count, ctx->max_smem, ctx->stream));
     ctx->launches += 1;     // row losses, then their mean
     return MCL_CUDA_OK;
 }

@@ -287,7 +287,7 @@ cudaError_t launch_token_logprobs_backward(const float* logits, const int* token
                                            size_t stride, float temperature, int sm_count, cudaStream_t stream);
 cudaError_t launch_distillation_loss(const float* logits, const int* teacher_ids, const float* teacher_logits, float* losses, float* out,
                                      float* row_stats, const float* grad_out, float* grad_logits, size_t rows, int cols, size_t stride,
-                                     int n_teacher, float temperature, int sm_count, cudaStream_t stream);
+                                     int n_teacher, float temperature, int* err_word, int sm_count, size_t max_smem, cudaStream_t stream);
 cudaError_t launch_distillation_loss_backward(const float* logits, const int* teacher_ids, const float* teacher_logits, const float* row_stats,
                                               const float* grad_out, float* grad_logits, size_t rows, int cols, size_t stride, int n_teacher,
                                               float temperature, int sm_count, cudaStream_t stream);

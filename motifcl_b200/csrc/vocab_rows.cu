@@ -8,6 +8,7 @@
 // Masked logits (-infinity, the lowest float) and rows with nothing left fall out of one clamp: 2^-150 is 0 in fp32, and
 // 0 * -150 is 0 where 0 * -infinity is not a number.
 #include "kernels.h"
+#include "tc_ptx.cuh"
 
 #include <cfloat>
 #include <cmath>
@@ -15,14 +16,14 @@
 namespace mcl {
 namespace {
 
-constexpr int kRowThreads = 512;
+constexpr int kRowThreads = 256;
 constexpr int kRowWarps = kRowThreads / 32;
+constexpr int kQuads = 4;              // of a thread in flight
 constexpr int kMaxList = kVocabListMax;
 constexpr int kMaxCluster = 8;
-constexpr int kCandidates = 2048;      // above a row's threshold, before the exact selection
-constexpr int kFinalists = 1024;       // a second threshold's
+constexpr int kHits = 1024;            // quads with a value above a row's first bound
+constexpr int kCandidates = 1024;      // values that reach its last one
 constexpr float kLn2 = 0.69314718f;    // ln 2 to fp32
-static_assert(kMaxCluster * kMaxList <= kCandidates, "the lists of a cluster's CTAs are candidates of its first one");
 
 // max(v, -150) that keeps NaN
 __device__ __forceinline__ float clamp_low(float v) {
@@ -66,12 +67,21 @@ struct Stats {
         if (x > m) raise(x, c);
         term(x, c);
     }
-    __device__ __forceinline__ void add(float4 v, float c) {
-        const float top = fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w));
-        if (top > m) raise(top, c);
-        term(v.x, c); term(v.y, c); term(v.z, c); term(v.w, c);
+    // of the lanes xor 1 .. `lanes` / 2
+    template <int LANES>
+    __device__ __forceinline__ void join(float c) {
+        float top = m;
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        raise(top, c);
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) {
+            s += __shfl_xor_sync(0xffffffffu, s, o);
+            if (ENTROPY) a += __shfl_xor_sync(0xffffffffu, a, o);
+        }
     }
 };
+__device__ __forceinline__ float top_of(float4 v) { return fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)); }
 
 // ---- a CTA's part of a row: `head` scalars up to a 16-byte boundary, n4 quads, the rest as scalars -----------------------
 struct Part {
@@ -83,28 +93,96 @@ struct Part {
         n4 = (n - head) >> 2;
     }
     __device__ __forceinline__ const float4* quads() const { return reinterpret_cast<const float4*>(p + head); }
-    // f(quad's index, its values) for the quads of this thread, four of them in flight
-    template <class F>
-    __device__ __forceinline__ void each_quad(F f) const {
-        constexpr int U = 4;
-        int i = threadIdx.x;
-        for (; i + (U - 1) * kRowThreads < n4; i += U * kRowThreads) {
-            float4 v[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u) v[u] = load_behind(quads() + i + u * kRowThreads);
-#pragma unroll
-            for (int u = 0; u < U; ++u) f(i + u * kRowThreads, v[u]);
-        }
-        for (; i < n4; i += kRowThreads) f(i, load_behind(quads() + i));
-    }
-    // f(place, value) for the scalars around them
-    template <class F>
-    __device__ __forceinline__ void each_loose(F f) const {
-        if ((int)threadIdx.x < n - 4 * n4) { const int at = loose(threadIdx.x); f(at, load_behind(p + at)); }
-    }
     // place of the i-th scalar outside the quads, i < n - 4 n4
     __device__ __forceinline__ int loose(int i) const { return i < head ? i : i + 4 * n4; }
 };
+
+// The quads of a thread: those at threadIdx.x modulo the threads, kQuads of them a step, a quarter of the part apart, so that the first step is a
+// sample of the part.  The distance depends on the part's length alone: a thread meets the same places whatever a row's alignment is.
+__device__ __forceinline__ int quarter_of(int n, int threads) { return (((n >> 2) + kQuads - 1) / kQuads + threads - 1) / threads * threads; }
+__device__ __forceinline__ void copy_async16(void* to, const void* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy_async4(void* to, const void* from) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int PENDING>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory"); }
+
+// Parts on their way: a thread copies the quads that it will work on itself, kAhead steps ahead and over the end of a part, so
+// that nothing waits for another thread and memory is busy while a row is finished.  part(i): the i-th of `items`, of at most `longest` logits.
+constexpr int kAhead = 2;
+template <int THREADS, class P>
+struct Stream {
+    float4* ring;                      // [kAhead][kQuads][THREADS]
+    const P& part;
+    Part at;                           // being fetched
+    size_t next_item, items;
+    int q, t, slot;
+    __device__ __forceinline__ Stream(void* shared, const P& parts, size_t count, int longest)
+        : ring(static_cast<float4*>(shared)), part(parts), at(parts(0)), next_item(0), items(count), q(quarter_of(longest, THREADS)), t(0), slot(0) {
+        for (int i = 0; i < kAhead; ++i) fetch(i);
+    }
+    __device__ __forceinline__ void fetch(int to) {
+        if (next_item < items && q > 0) {
+#pragma unroll
+            for (int u = 0; u < kQuads; ++u) {
+                const int i = u * q + t + (int)threadIdx.x;
+                if (i < at.n4) copy_async16(ring + (to * kQuads + u) * THREADS + threadIdx.x, at.quads() + i);
+            }
+            t += THREADS;
+            if (t >= q) {
+                t = 0;
+                if (++next_item < items) at = part(next_item);
+            }
+        }
+        copies_end();
+    }
+    // step `now` of a part with n4 quads: -infinity behind the end.  next() follows when the values have been used
+    __device__ __forceinline__ void take(int now, int n4, float4 (&v)[kQuads]) {
+        copies_wait<kAhead - 1>();
+#pragma unroll
+        for (int u = 0; u < kQuads; ++u)
+            v[u] = u * q + now + (int)threadIdx.x < n4 ? ring[(slot * kQuads + u) * THREADS + threadIdx.x] : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+    }
+    __device__ __forceinline__ void next() {
+        fetch(slot);
+        slot = slot + 1 < kAhead ? slot + 1 : 0;
+    }
+};
+constexpr size_t kStreamBytes = (size_t)kAhead * kQuads * kRowThreads * sizeof(float4);
+
+// g[i] = f(x[i]) over a part; v is the first step, loaded by the caller ahead of what f waits for.  By loads and stores of the threads themselves:
+// asynchronous copies behind stores wait in the same queue (4096 x 32000: 184 us, 163 so).
+__device__ __forceinline__ void load_step(const Part& part, int q, int t, float4 (&v)[kQuads]) {
+#pragma unroll
+    for (int u = 0; u < kQuads; ++u) {
+        const int i = u * q + t + (int)threadIdx.x;
+        if (i < part.n4) v[u] = load_behind(part.quads() + i);
+    }
+}
+template <int THREADS, class F>
+__device__ __forceinline__ void write_part(const Part& part, int q, float* g, float4 (&v)[kQuads], float loose, F f) {
+    const bool vec = ((reinterpret_cast<uintptr_t>(g) ^ reinterpret_cast<uintptr_t>(part.p)) & 15) == 0;
+    float4 next[kQuads];
+#pragma unroll 1
+    for (int t = 0; t < q; t += THREADS) {
+        if (t + THREADS < q) load_step(part, q, t + THREADS, next);
+#pragma unroll
+        for (int u = 0; u < kQuads; ++u) {
+            const int i = u * q + t + (int)threadIdx.x;
+            if (i >= part.n4) continue;
+            float* to = g + part.head + 4 * i;
+            const float4 o = make_float4(f(v[u].x), f(v[u].y), f(v[u].z), f(v[u].w));
+            if (vec) *reinterpret_cast<float4*>(to) = o;
+            else { to[0] = o.x; to[1] = o.y; to[2] = o.z; to[3] = o.w; }
+        }
+#pragma unroll
+        for (int u = 0; u < kQuads; ++u) v[u] = next[u];
+    }
+    if ((int)threadIdx.x < part.n - 4 * part.n4) g[part.loose(threadIdx.x)] = f(loose);
+}
 
 // ---- selection of the largest ------------------------------------------------------------------------------------------
 // A candidate is one whole number: the logit's bits in an order that is the floats' (equal zeros equal), then the place, lower ones larger.
@@ -118,16 +196,19 @@ __device__ __forceinline__ unsigned long long candidate(float v, int at) {
 }
 struct Selection {
     unsigned long long list[kCandidates];
-    unsigned long long last[kFinalists];
     unsigned long long best[kMaxList];     // largest first
-    uint32_t bound[kRowWarps];
-    int count, finalists, scanned[kRowWarps];
+    int hits[kHits];                       // quads
+    uint32_t bound[2][kRowWarps];
+    int n_hits[2], n_list[2], scanned[kRowWarps];
 };
+// behind it, where a row has a cluster: the best of all its CTAs, kMaxList places each, in the first one
+
 // A bound that at least k of the threads' values reach: every warp's r-th largest, r = k / warps rounded up, and of those the smallest.
-// All threads; one barrier inside, one more before the next call.
+// All threads; one barrier inside; calls alternate between the two `bound`s.
 __device__ __forceinline__ uint32_t bound_of(uint32_t mine, int k, uint32_t* bound) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     uint32_t top = 0;
+#pragma unroll 1
     for (int r = (k + kRowWarps - 1) / kRowWarps; r > 0; --r) {
         top = __reduce_max_sync(0xffffffffu, mine);
         const unsigned at = __ballot_sync(0xffffffffu, mine == top);
@@ -137,59 +218,101 @@ __device__ __forceinline__ uint32_t bound_of(uint32_t mine, int k, uint32_t* bou
     __syncthreads();
     return __reduce_min_sync(0xffffffffu, bound[lane & (kRowWarps - 1)]);
 }
-// The k largest of list[0 .. n) to best[], in order; k <= n <= kCandidates.  All threads; ends with a barrier.
-__device__ __forceinline__ void select_best(Selection& z, int n, int k) {
-    const unsigned long long* from = z.list;
-    int m = n;
-    if (n > 2 * k) {                          // ranks cost n^2: first those below a bound go
-        uint32_t mine = 0;
-        for (int i = threadIdx.x; i < n; i += kRowThreads) mine = max(mine, (uint32_t)(z.list[i] >> 32));
-        if (threadIdx.x == 0) z.finalists = 0;
-        const uint32_t least = bound_of(mine, k, z.bound);       // 0 where threads without a candidate are among them
-        for (int i = threadIdx.x; i < n; i += kRowThreads) {
-            const unsigned long long v = z.list[i];
-            if ((uint32_t)(v >> 32) < least) continue;
-            const int at = atomicAdd(&z.finalists, 1);
-            if (at < kFinalists) z.last[at] = v;
-        }
-        __syncthreads();
-        if (z.finalists <= kFinalists) { from = z.last; m = z.finalists; }
-    }
-    for (int i = threadIdx.x; i < m; i += kRowThreads) {
-        const unsigned long long v = from[i];
-        int rank = 0;
-#pragma unroll 4
-        for (int j = 0; j < m; ++j) rank += from[j] > v;         // no two are equal: their places differ
-        if (rank < k) z.best[rank] = v;
-    }
-    __syncthreads();
-}
-
-// g[i] = f(x[i]) over a part; g may be x itself
+// f(rank, candidate) for the k largest of list[0 .. n).  No two candidates are equal: their places differ.  The fewer they are, the more lanes
+// count for one of them.
 template <class F>
-__device__ __forceinline__ void write_part(const Part& part, float* g, F f) {
-    if (((reinterpret_cast<uintptr_t>(g) ^ reinterpret_cast<uintptr_t>(part.p)) & 15) == 0) {
-        float4* g4 = reinterpret_cast<float4*>(g + part.head);
-        part.each_quad([&](int i, float4 v) { g4[i] = make_float4(f(v.x), f(v.y), f(v.z), f(v.w)); });
-    } else {
-        float* gq = g + part.head;
-        part.each_quad([&](int i, float4 v) { gq[4 * i] = f(v.x); gq[4 * i + 1] = f(v.y); gq[4 * i + 2] = f(v.z); gq[4 * i + 3] = f(v.w); });
+__device__ __forceinline__ void each_best(const unsigned long long* list, int n, int k, F f) {
+    const int log = n <= 32 ? 3 : n <= 64 ? 2 : n <= 128 ? 1 : 0, lanes = 1 << log;
+    const int part = threadIdx.x & (lanes - 1);
+#pragma unroll 1
+    for (int first = 0; first < n; first += kRowThreads >> log) {
+        const int i = first + (threadIdx.x >> log);
+        if (first + (((int)threadIdx.x & ~31) >> log) >= n) break;           // the whole warp
+        const unsigned long long v = list[min(i, n - 1)];
+        int rank = 0, j = part;
+#pragma unroll 1
+        for (; j + 3 * lanes < n; j += 4 * lanes) {
+            unsigned long long w[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) w[u] = list[j + u * lanes];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) rank += w[u] > v;
+        }
+#pragma unroll 1
+        for (; j < n; j += lanes) rank += list[j] > v;
+#pragma unroll 1
+        for (int o = 1; o < lanes; o <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
+        if (part == 0 && i < n && rank < k) f(rank, v);
     }
-    part.each_loose([&](int at, float v) { g[at] = f(v); });
 }
-__device__ __forceinline__ void clear_part(float* g, int n) {
-    const int head = min(n, (int)((16 - (reinterpret_cast<uintptr_t>(g) & 15)) & 15) >> 2), n4 = (n - head) >> 2;
-    for (int i = threadIdx.x; i < n4; i += kRowThreads) reinterpret_cast<float4*>(g + head)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-    if ((int)threadIdx.x < n - 4 * n4) g[(int)threadIdx.x < head ? threadIdx.x : threadIdx.x + 4 * n4] = 0.0f;
+// To list: the values of v, a quad at `at`, that reach `least`, or are above it (strict).
+__device__ __forceinline__ void take(Selection& z, int* count, float v, int at, float least, bool strict) {
+    if (!(v >= least) || (strict && v == least)) return;
+    const int i = atomicAdd(count, 1);
+    if (i < kCandidates) z.list[i] = candidate(v, at);
+}
+// ... of a whole part, from memory.  All threads.
+__device__ __noinline__ void take_part(Selection& z, int* count, const float* p, int n, int c0, float least, bool strict) {
+    const Part part(p, n);
+#pragma unroll 1
+    for (int t = threadIdx.x; t < part.n4; t += kQuads * kRowThreads) {
+        float4 v[kQuads];
+#pragma unroll
+        for (int u = 0; u < kQuads; ++u) v[u] = load_behind(part.quads() + min(t + u * kRowThreads, part.n4 - 1));
+#pragma unroll
+        for (int u = 0; u < kQuads; ++u) {
+            if (t + u * kRowThreads >= part.n4 || !(top_of(v[u]) >= least)) continue;
+            const int at = c0 + part.head + 4 * (t + u * kRowThreads);
+            take(z, count, v[u].x, at, least, strict); take(z, count, v[u].y, at + 1, least, strict);
+            take(z, count, v[u].z, at + 2, least, strict); take(z, count, v[u].w, at + 3, least, strict);
+        }
+    }
+    if ((int)threadIdx.x < part.n - 4 * part.n4) { const int at = part.loose(threadIdx.x); take(z, count, load_behind(part.p + at), c0 + at, least, strict); }
+}
+// The first of those equal to `least` to list[n .. k_part).
+__device__ __noinline__ void fill_equal(Selection& z, const float* p, int part_n, int c0, float least, int n, int k_part) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll 1
+    for (int c = 0; c < part_n && n < k_part; c += kRowThreads) {
+        const int at = c + threadIdx.x;
+        const bool hit = at < part_n && load_behind(p + at) == least;
+        const unsigned hits = __ballot_sync(0xffffffffu, hit);
+        if (lane == 0) z.scanned[warp] = __popc(hits);
+        __syncthreads();
+        int before = n, all = n;
+        for (int w = 0; w < kRowWarps; ++w) { if (w < warp) before += z.scanned[w]; all += z.scanned[w]; }
+        before += __popc(hits & ((1u << lane) - 1));
+        if (hit && before < k_part) z.list[before] = candidate(least, c0 + at);
+        n = min(all, k_part);
+        __syncthreads();
+    }
+}
+// Many equal values, or many large ones in few threads: the values above `least` alone, and the first of those equal to it where they are too few;
+// while there is no room for them, the k-th largest of those that there is room for becomes `least` (k of the part reach it, and each of them is
+// above the old one).  At least k_part of the part reach `least`.  Returns their number.
+__device__ __noinline__ int take_few(Selection& z, int* count, const float* p, int part_n, int c0, float least, int k, int k_part) {
+#pragma unroll 1
+    for (;;) {
+        __syncthreads();
+        if (threadIdx.x == 0) *count = 0;
+        __syncthreads();
+        take_part(z, count, p, part_n, c0, least, true);
+        __syncthreads();
+        const int n = *count;
+        if (n <= kCandidates) {
+            if (n < k_part) fill_equal(z, p, part_n, c0, least, n, k_part);
+            return max(n, k_part);
+        }
+        each_best(z.list, kCandidates, k, [&](int rank, unsigned long long v) { if (rank == k - 1) z.best[0] = v; });
+        __syncthreads();
+        least = unordered((uint32_t)(z.best[0] >> 32));
+    }
 }
 
 // ---- what a row's CTAs share -------------------------------------------------------------------------------------------
 struct RowShared {
-    float wm[kRowWarps], ws[kRowWarps], wa[kRowWarps];
-    float cm[kMaxCluster], cs[kMaxCluster], ca[kMaxCluster];       // written by the cluster's CTAs
-    float t[kMaxList], log_t[kMaxList], x[kMaxList];                // the teacher's list: probabilities, their logarithms, the student's logits there
-    int id[kMaxList];                                               // -1: no entry
-    float t_sum;                                                    // of the exponentials; 0: an empty list
+    float wm[2][kRowWarps], ws[2][kRowWarps], wa[2][kRowWarps];    // of this row and of the one before, which may still be read
+    float cm[2][kMaxCluster], cs[2][kMaxCluster], ca[2][kMaxCluster];       // written by the cluster's CTAs
 };
 __device__ __forceinline__ uint32_t cluster_address(const void* shared, int rank) {
     uint32_t to;
@@ -217,213 +340,569 @@ struct VocabRows {
     float* losses;
     const float* grad_out;             // with grad_logits
     float* grad_logits;
+    int* err_word;                     // where a bounded wait gives up
 };
 
-// The teacher's list of a row by one warp: probabilities of its entries among themselves, and the student's logits there.
-__device__ __forceinline__ void read_list(const VocabRows& p, size_t row, RowShared& sh) {
-    const int lane = threadIdx.x & 31;
-    const float* x = p.logits + row * p.stride;
+// ---- a teacher's lists, by one warp -----------------------------------------------------------------------------------
+// It goes ahead of the others: the ids and logits of the item after the next and the student's logits at the ids of the next are on their way
+// (asynchronous copies; a loop of loads would wait for each) while it works on the lists before.
+struct __align__(16) TeacherList {
+    int id[kMaxList];                  // outside [0, cols): no entry
+    float t[kMaxList], log_t[kMaxList], x[kMaxList];                // probabilities, their logarithms, the student's logits
+    float g[kMaxList];                 // the listed tokens' gradients (list_take_off)
+    float sum;                         // of the exponentials; 0: an empty list
+    bool twice;                        // a token is named more than once
+};
+template <class P>
+__device__ __forceinline__ void list_fetch(TeacherList& l, const P& p, size_t row) {
     const size_t at = row * (size_t)p.n_teacher;
-    float top = -FLT_MAX, sum = 0.0f;
-    for (int i = lane; i < p.n_teacher; i += 32) {
-        const int id = load_behind(p.teacher_ids + at + i);
-        const bool in = id >= 0 && id < p.cols;
-        const float v = in ? load_behind(p.teacher_logits + at + i) : -INFINITY;
-        sh.id[i] = in ? id : -1;
-        sh.t[i] = sh.log_t[i] = v;
-        sh.x[i] = in ? load_behind(x + id) : 0.0f;
-        top = fmaxf(top, v);
+    for (int i = threadIdx.x & 31; i < p.n_teacher; i += 32) {
+        copy_async4(&l.id[i], p.teacher_ids + at + i);
+        copy_async4(&l.t[i], p.teacher_logits + at + i);
     }
+}
+template <class P>
+__device__ __forceinline__ void list_gather(TeacherList& l, const P& p, size_t row) {
+    const float* x = p.logits + row * p.stride;
+    for (int i = threadIdx.x & 31; i < p.n_teacher; i += 32) {
+        const int id = l.id[i];
+        if (id >= 0 && id < p.cols) copy_async4(&l.x[i], x + id);
+        else l.t[i] = -INFINITY;
+    }
+}
+// Probabilities t = exp2((a - top) c) / sum of the logits a.
+template <class P>
+__device__ __forceinline__ void list_terms(TeacherList& l, const P& p) {
+    const int lane = threadIdx.x & 31;
+    float top = -FLT_MAX, sum = 0.0f;
+    for (int i = lane; i < p.n_teacher; i += 32) top = fmaxf(top, l.t[i]);
     top = warp_top(top);
-    for (int i = lane; i < p.n_teacher; i += 32) sum += exp2_fast(clamp_low((sh.t[i] - top) * p.c));
+    for (int i = lane; i < p.n_teacher; i += 32) {
+        const float d = l.t[i] - top, e = exp2_fast(clamp_low(d * p.c));
+        l.log_t[i] = d;
+        l.t[i] = e;
+        sum += e;
+    }
     sum = warp_add(sum);
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum, log_sum = logf(sum);
-    if (lane == 0) sh.t_sum = sum;
-    for (int i = lane; i < p.n_teacher; i += 32) {
-        const float d = clamp_low((sh.t[i] - top) * p.c);
-        sh.t[i] = exp2_fast(d) * inv;
-        sh.log_t[i] = (sh.log_t[i] - top) * p.inv_t - log_sum;
+    for (int i = lane; i < p.n_teacher; i += 32) { l.t[i] *= inv; l.log_t[i] = l.log_t[i] * p.inv_t - log_sum; }
+    if (lane == 0) l.sum = sum;
+    __syncwarp();
+}
+// Takes the listed tokens' probabilities, times `up`, off their gradients: where(i) is the gradient of entry i, or null.  Entries that name the same
+// token find out through it: each leaves its number there, and one of them finds its own; that one takes off all of theirs, in their order.
+template <class W>
+__device__ __forceinline__ void list_take_off(TeacherList& l, int n, float up, W where) {
+    const int lane = threadIdx.x & 31;
+    for (int i = lane; i < n; i += 32) {
+        volatile float* g = where(i);
+        if (g != nullptr) l.g[i] = *g;
+    }
+    __syncwarp();
+    for (int i = lane; i < n; i += 32) {
+        volatile int* g = reinterpret_cast<volatile int*>(where(i));
+        if (g != nullptr) *g = i;
+    }
+    __syncwarp();
+    unsigned last = 0;                 // bit j: entry lane + 32 j found its number
+    bool twice = false;
+    for (int i = lane, j = 0; i < n; i += 32, ++j) {
+        volatile int* g = reinterpret_cast<volatile int*>(where(i));
+        if (g == nullptr) continue;
+        if (*g == i) last |= 1u << j;
+        else twice = true;
+    }
+    twice = __any_sync(0xffffffffu, twice);
+    for (int i = lane, j = 0; i < n; i += 32, ++j) {
+        if (!(last >> j & 1u)) continue;
+        float t = l.t[i];
+        if (twice) {
+            t = 0.0f;
+            for (int o = 0; o < n; ++o)
+                if (l.id[o] == l.id[i]) t += l.t[o];
+        }
+        *where(i) = l.g[i] - t * up;
     }
     __syncwarp();
 }
-// g[id] of the listed tokens in [c0, c0 + cn), behind the rest of g: the first entry that names one writes it, with all that name it, in their order
 template <class F>
-__device__ __forceinline__ void write_listed(const RowShared& sh, int n, float* g, int c0, int cn, float up, F value) {
-    const int id = (int)threadIdx.x < n ? sh.id[threadIdx.x] : -1;
-    if (id < c0 || id >= c0 + cn) return;
-    float t = 0.0f;
-    bool first = true;
-    for (int j = 0; j < n; ++j)
-        if (sh.id[j] == id) { t += sh.t[j]; first = first && j >= (int)threadIdx.x; }
-    if (first) g[id - c0] = value(sh.x[threadIdx.x]) - t * up;
+__device__ __forceinline__ float list_loss(const TeacherList& l, int n, F log_prob) {
+    float loss = 0.0f;
+    for (int i = threadIdx.x & 31; i < n; i += 32) {
+        const float t = l.t[i];
+        if (t != 0.0f) loss += t * (l.log_t[i] - log_prob(l.x[i]));
+    }
+    return warp_add(loss);
+}
+// Whether two entries of a list name the same token.  All lanes take part in every step: what a lane has found keeps it from none.
+template <class P>
+__device__ __forceinline__ bool list_twice(const TeacherList& l, const P& p) {
+    const int lane = threadIdx.x & 31;
+    bool twice = false;
+#pragma unroll 1
+    for (int i = 0; i < p.n_teacher; i += 32) {
+        const int id = i + lane < p.n_teacher ? l.id[i + lane] : -1;
+        const bool entry = id >= 0 && id < p.cols;
+        const unsigned same = __match_any_sync(0xffffffffu, entry ? id : -1 - lane);
+        twice |= entry && same != 1u << lane;
+#pragma unroll 1
+        for (int j = i + 32; j < p.n_teacher; j += 4) {           // against each entry of the groups of 32 behind it
+            const int4 other = *reinterpret_cast<const int4*>(&l.id[j]);
+            const bool found = id == other.x || (id == other.y && j + 1 < p.n_teacher) || (id == other.z && j + 2 < p.n_teacher) || (id == other.w && j + 3 < p.n_teacher);
+            twice |= entry && found;
+        }
+    }
+    return __any_sync(0xffffffffu, twice);
+}
+// g[id] of the listed tokens in [c0, c0 + cn), behind the rest of g, from the student's logits: the first entry that names a token takes all of
+// its entries' probabilities off, in their order.
+template <class F>
+__device__ __forceinline__ void list_write(const TeacherList& l, int n, float* g, int c0, int cn, float up, F value) {
+    for (int i = threadIdx.x & 31; i < n; i += 32) {
+        const int id = l.id[i];
+        if (id < c0 || id - c0 >= cn) continue;
+        float t = l.t[i];
+        if (l.twice) {
+            bool first = true;
+            t = 0.0f;
+            for (int j = 0; j < n; ++j)
+                if (l.id[j] == id) { t += l.t[j]; first = first && j >= i; }
+            if (!first) continue;
+        }
+        g[id - c0] = value(l.x[i]) - t * up;
+    }
+}
+// The lists of items 0, 1, ... of a CTA: row(i) is an item's row.
+template <int LISTS, class P, class R>
+struct ListWarp {
+    TeacherList* lists;                // LISTS of them, three or more
+    const P& p;
+    size_t items;                      // of this CTA
+    R row;
+    __device__ __forceinline__ TeacherList& of(size_t i) { return lists[i % LISTS]; }
+    // before the first item
+    __device__ __forceinline__ void start() {
+        if (items == 0) return;
+        list_fetch(of(0), p, row(0));
+        if (items > 1) list_fetch(of(1), p, row(1));
+        copies_end();
+        copies_wait<0>();
+        __syncwarp();
+        list_gather(of(0), p, row(0));
+        copies_end();
+        __syncwarp();
+        list_terms(of(0), p);
+        const bool twice = list_twice(of(0), p);
+        if ((threadIdx.x & 31) == 0) of(0).twice = twice;
+        copies_wait<0>();
+        __syncwarp();
+    }
+    // while item i is at work and all of item i - 1 is done: the next one's terms and student logits
+    __device__ __forceinline__ void ahead(size_t i) {
+        copies_wait<0>();
+        __syncwarp();
+        if (i + 1 < items) list_gather(of(i + 1), p, row(i + 1));
+        if (i + 2 < items) list_fetch(of(i + 2), p, row(i + 2));
+        copies_end();
+        __syncwarp();
+        if (i + 1 < items) {
+            list_terms(of(i + 1), p);
+            const bool twice = list_twice(of(i + 1), p);
+            if ((threadIdx.x & 31) == 0) of(i + 1).twice = twice;
+        }
+    }
+    // before an item's student logits are used
+    __device__ __forceinline__ void arrived() {
+        copies_wait<0>();
+        __syncwarp();
+    }
+};
+
+// The statistics that the backward call takes: no sum where the row has no entries, none that is a number where its list is none.
+__device__ __forceinline__ float gradient_sum(float s, float list_sum) { return list_sum == 0.0f ? 0.0f : list_sum == list_sum ? s : list_sum; }
+__device__ __forceinline__ void list_result(const VocabRows& p, const TeacherList& l, size_t row, float m, float s, float loss) {
+    if ((threadIdx.x & 31) != 0) return;
+    p.losses[row] = loss;
+    if (p.row_stats != nullptr) { p.row_stats[2 * row] = m; p.row_stats[2 * row + 1] = gradient_sum(s, l.sum); }
 }
 
 // One row at a time on a CTA, or a row on a cluster's CTAs where there are few.
-template <bool ENTROPY, bool TOP, bool DISTILL>
-__global__ void __launch_bounds__(kRowThreads) vocab_rows_kernel(VocabRows p) {
+// TOP: a thread's first step is a sample of the row; the quads with something above the bound that it gives are noted as the row goes by, and
+// looked at again under the bound of all that the threads have seen.
+// LIST, GRAD: the last warp has the teacher's lists and forms the losses; the row goes by a second time (out of L2), becomes its gradient, and that
+// warp takes the listed tokens' probabilities off it while the next row is at work.
+enum RowWork { kPlain, kTop, kList, kGrad };
+template <bool ENTROPY, RowWork WORK>
+__global__ void __launch_bounds__(kRowThreads, 4) vocab_rows_kernel(VocabRows p) {
+    constexpr bool TOP = WORK == kTop, DISTILL = WORK == kList || WORK == kGrad, GRAD = WORK == kGrad;
+    constexpr int THREADS = kRowThreads - (DISTILL ? 32 : 0), WARPS = THREADS / 32;       // that work on rows
     grid_release();
     extern __shared__ __align__(16) unsigned char dynamic[];
-    Selection& z = *reinterpret_cast<Selection*>(dynamic);       // TOP
+    Selection& z = *reinterpret_cast<Selection*>(dynamic + kStreamBytes);       // TOP
+    unsigned long long* gathered = reinterpret_cast<unsigned long long*>(dynamic + kStreamBytes + sizeof(Selection));
+    TeacherList* lists = reinterpret_cast<TeacherList*>(dynamic + kStreamBytes);                   // DISTILL
     __shared__ RowShared sh;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int ranks = p.cluster, rank = ranks > 1 ? (int)(blockIdx.x % ranks) : 0;
     const int per = ((p.cols + ranks - 1) / ranks + 3) & ~3;
     const int c0 = min(p.cols, rank * per), cn = min(p.cols, c0 + per) - c0;
+    const size_t first = blockIdx.x / ranks, step = gridDim.x / ranks, mine = (p.rows - first + step - 1) / step;
+    const int k = p.n_top, k_part = min(k, cn);
     if (ranks > 1) { cluster_arrive(); cluster_wait(); }          // every CTA of the cluster runs
+    if (TOP && threadIdx.x == 0) z.n_hits[0] = z.n_hits[1] = 0;
+    if (DISTILL && threadIdx.x == 0)                              // the one that joins statistics of WARPS takes a power of two of them
+        for (int w = WARPS; w < kRowWarps; ++w) { sh.wm[0][w] = sh.wm[1][w] = -FLT_MAX; sh.ws[0][w] = sh.ws[1][w] = 0.0f; }
     grid_wait();
-    for (size_t row = blockIdx.x / ranks; row < p.rows; row += gridDim.x / ranks) {
+    const bool of_lists = DISTILL && warp == WARPS;
+    auto row_of = [&](size_t i) { return first + i * step; };
+    auto part_of = [&](size_t i) { return Part(p.logits + row_of(i) * p.stride + c0, cn); };
+    ListWarp<3, VocabRows, decltype(row_of)> list_warp = {lists, p, mine, row_of};
+    if (of_lists) list_warp.start();
+    Stream<THREADS, decltype(part_of)> stream(dynamic, part_of, of_lists ? 0 : mine, cn);
+    const int q = stream.q;
+    const float up = GRAD ? load_behind(p.grad_out) * p.inv_t / (float)p.rows : 0.0f;
+    // GRAD, of the row before too, whose listed tokens are written when all of its gradient is
+    float gm = 0.0f, gf = 0.0f;
+    bool none = true;
+    auto value = [&](float v) { return none ? 0.0f : exp2_fast(clamp_low((v - gm) * p.c)) * gf; };
+    auto write_behind = [&](size_t item) {
+        if (!none) list_write(list_warp.of(item), p.n_teacher, p.grad_logits + row_of(item) * p.stride + c0, c0, cn, up, value);
+    };
+    for (size_t item = 0; item < mine; ++item) {
+        const size_t row = row_of(item);
+        const int turn = (int)(item & 1);
         const float* x = p.logits + row * p.stride;
         const Part part(x + c0, cn);
-        if (DISTILL && warp == 0) read_list(p, row, sh);
-        float x_token = 0.0f;
-        int token = -1;
-        if (!DISTILL && p.tokens != nullptr && threadIdx.x == 0 && rank == 0) {
-            token = load_behind(p.tokens + row);
-            if (token < 0 || token >= p.cols) token = -1;
-            else x_token = load_behind(x + token);
-        }
-        // the row's statistics
         Stats<ENTROPY> st;
-        part.each_quad([&](int, float4 v) { st.add(v, p.c); });
-        part.each_loose([&](int, float v) { st.add(v, p.c); });
-        const float mine = st.m == -FLT_MAX ? -INFINITY : st.m;   // TOP: this thread's largest is no less
-        float m = warp_top(st.m);
-        if (lane == 0) sh.wm[warp] = m;
-        __syncthreads();
-        m = warp_top(sh.wm[lane & (kRowWarps - 1)]);
-        st.raise(m, p.c);
-        float s = warp_add(st.s), a = ENTROPY ? warp_add(st.a) : 0.0f;
-        if (lane == 0) { sh.ws[warp] = s; if (ENTROPY) sh.wa[warp] = a; }
-        __syncthreads();
-        s = a = 0.0f;
+        float over = INFINITY, x_token = 0.0f, loose = -INFINITY;
+        int token = -1;
+        const bool has_loose = (int)threadIdx.x < part.n - 4 * part.n4;
+        float4 again[kQuads];                                     // GRAD: the first step a second time
+        if (!of_lists) {
+            if (has_loose) loose = load_behind(part.p + part.loose(threadIdx.x));
+            if (!DISTILL && p.tokens != nullptr && threadIdx.x == 0 && rank == 0) {
+                token = load_behind(p.tokens + row);
+                if (token < 0 || token >= p.cols) token = -1;
+                else x_token = load_behind(x + token);
+            }
+#pragma unroll 1
+            for (int t = 0; t < q; t += THREADS) {
+                float4 v[kQuads];
+                stream.take(t, part.n4, v);
+                float top = top_of(v[0]);
 #pragma unroll
-        for (int w = 0; w < kRowWarps; ++w) { s += sh.ws[w]; if (ENTROPY) a += sh.wa[w]; }
+                for (int u = 1; u < kQuads; ++u) top = fmaxf(top, top_of(v[u]));
+                if (top > st.m) st.raise(top, p.c);
+                stream.next();
+#pragma unroll
+                for (int u = 0; u < kQuads; ++u) { st.term(v[u].x, p.c); st.term(v[u].y, p.c); st.term(v[u].z, p.c); st.term(v[u].w, p.c); }
+                if (TOP) {
+                    if (t == 0 && THREADS < q)                    // this thread's largest is no less than st.m, or -infinity
+                        over = unordered(max(bound_of(ordered(st.m == -FLT_MAX ? -INFINITY : st.m), k, z.bound[0]), ordered(-INFINITY)));
+                    if (top > over) {
+                        unsigned which = 0;
+#pragma unroll
+                        for (int u = 0; u < kQuads; ++u) which |= top_of(v[u]) > over ? 1u << u : 0u;
+                        int at = atomicAdd(&z.n_hits[turn], __popc(which));
+#pragma unroll
+                        for (int u = 0; u < kQuads; ++u)
+                            if (which >> u & 1u) { if (at < kHits) z.hits[at] = u * q + t + (int)threadIdx.x; ++at; }
+                    }
+                }
+            }
+            st.add(loose, p.c);
+            if (GRAD) load_step(part, q, 0, again);
+        }
+        float least = -INFINITY;
+        if (TOP) {
+            if (threadIdx.x == 0) z.n_list[turn] = 0;
+            least = unordered(max(bound_of(ordered(st.m == -FLT_MAX ? -INFINITY : st.m), k, z.bound[1]), ordered(-INFINITY)));
+        }
+        if (!of_lists) {
+            st.template join<32>(p.c);
+            if (lane == 0) { sh.wm[turn][warp] = st.m; sh.ws[turn][warp] = st.s; if (ENTROPY) sh.wa[turn][warp] = st.a; }
+        }
+        if (TOP) {
+            const int hits = z.n_hits[turn];
+            int* count = &z.n_list[turn];
+            const bool strict = !(least > over);                  // among the quads that were not noted some may equal it
+            if (hits > kHits || q <= THREADS) take_part(z, count, part.p, part.n, c0, least, false);
+            else {
+#pragma unroll 1
+                for (int i = threadIdx.x; i < hits; i += kQuads * kRowThreads) {
+                    int quad[kQuads];
+                    float4 v[kQuads];
+#pragma unroll
+                    for (int u = 0; u < kQuads; ++u) quad[u] = z.hits[min(i + u * kRowThreads, hits - 1)];
+#pragma unroll
+                    for (int u = 0; u < kQuads; ++u) v[u] = load_behind(part.quads() + quad[u]);
+#pragma unroll
+                    for (int u = 0; u < kQuads; ++u) {
+                        if (i + u * kRowThreads >= hits || !(top_of(v[u]) >= least)) continue;
+                        const int at = c0 + part.head + 4 * quad[u];
+                        take(z, count, v[u].x, at, least, strict); take(z, count, v[u].y, at + 1, least, strict);
+                        take(z, count, v[u].z, at + 2, least, strict); take(z, count, v[u].w, at + 3, least, strict);
+                    }
+                }
+                if (has_loose) take(z, count, loose, c0 + part.loose(threadIdx.x), least, strict);
+            }
+        }
+        if (of_lists) list_warp.arrived();                        // before anything of this row may become its gradient (grad_logits == logits)
+        __syncthreads();                                          // GRAD: and all of the gradient of the row before is there
+        if (GRAD && of_lists && item > 0) write_behind(item - 1);
+        st.m = sh.wm[turn][lane & (kRowWarps - 1)];
+        st.s = sh.ws[turn][lane & (kRowWarps - 1)];
+        if (ENTROPY) st.a = sh.wa[turn][lane & (kRowWarps - 1)];
+        st.template join<kRowWarps>(p.c);
+        int n = 0;
+        if (TOP) {
+            if (threadIdx.x == 0) z.n_hits[turn] = 0;             // for the row after the next
+            n = z.n_list[turn];
+            if (!(st.s == st.s)) n = 0;                           // not a number: its places are not looked at
+            else if (n > kCandidates || n < k_part) n = take_few(z, &z.n_list[turn], part.p, part.n, c0, least, k, k_part);
+        }
         if (ranks > 1) {
-            if ((int)threadIdx.x < ranks) {
-                asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_address(&sh.cm[rank], threadIdx.x)), "f"(m) : "memory");
-                asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_address(&sh.cs[rank], threadIdx.x)), "f"(s) : "memory");
-                asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_address(&sh.ca[rank], threadIdx.x)), "f"(a) : "memory");
+            // the first CTA gets all statistics and every part's best
+            if (TOP) {
+                each_best(z.list, n, k_part, [&](int r, unsigned long long c) { z.best[r] = c; });
+                __syncthreads();
+                if ((int)threadIdx.x < k)
+                    asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(cluster_address(&gathered[rank * k + threadIdx.x], 0)),
+                                 "l"((int)threadIdx.x < min(n, k_part) ? z.best[threadIdx.x] : 0ull) : "memory");       // 0: below every candidate
+            }
+            if ((int)threadIdx.x < (GRAD ? ranks : 1)) {          // GRAD: all of them
+                asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_address(&sh.cm[turn][rank], threadIdx.x)), "f"(st.m) : "memory");
+                asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_address(&sh.cs[turn][rank], threadIdx.x)), "f"(st.s) : "memory");
+                if (ENTROPY) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_address(&sh.ca[turn][rank], threadIdx.x)), "f"(st.a) : "memory");
             }
             cluster_arrive();
             cluster_wait();
+            if (!GRAD && rank > 0) return;                        // a cluster has one row (launch_forward)
             Stats<ENTROPY> all;
-            for (int r = 0; r < ranks; ++r) all.m = fmaxf(all.m, sh.cm[r]);
+            for (int r = 0; r < ranks; ++r) all.m = fmaxf(all.m, sh.cm[turn][r]);
             for (int r = 0; r < ranks; ++r) {
                 Stats<ENTROPY> one;
-                one.m = sh.cm[r]; one.s = sh.cs[r]; one.a = sh.ca[r];
+                one.m = sh.cm[turn][r]; one.s = sh.cs[turn][r];
+                if (ENTROPY) one.a = sh.ca[turn][r];
                 one.raise(all.m, p.c);
                 all.s += one.s; all.a += one.a;
             }
-            m = all.m; s = all.s; a = all.a;
+            st = all;
         }
-        const float log_s = logf(s);
-        auto log_prob = [&](float v) { return s == 0.0f ? -INFINITY : (v - m) * p.inv_t - log_s; };      // s == 0: nothing is left of the row
-        if (threadIdx.x == 0 && rank == 0) {
+        const float m = st.m, s = st.s, log_s = logf(s);
+        auto log_prob = [&](float value) { return s == 0.0f ? -INFINITY : (value - m) * p.inv_t - log_s; };      // s == 0: nothing is left of the row
+        if (!DISTILL && threadIdx.x == 0) {
             if (p.row_stats != nullptr) { p.row_stats[2 * row] = m; p.row_stats[2 * row + 1] = s; }
-            if (!DISTILL && p.logprobs != nullptr) p.logprobs[row] = token < 0 ? 0.0f : log_prob(x_token);
-            if (ENTROPY && p.entropy != nullptr) p.entropy[row] = s == 0.0f ? 0.0f : log_s - a / s * kLn2;
+            if (p.logprobs != nullptr) p.logprobs[row] = token < 0 ? 0.0f : log_prob(x_token);
+            if (ENTROPY) p.entropy[row] = s == 0.0f ? 0.0f : log_s - st.a / s * kLn2;
         }
         if (TOP) {
-            // Every thread has its largest; at least n_top of the row reach their bound.  What is above it is collected, equal ones are looked for
-            // in order only where those are too few.  More than fit (values above the bound in few threads) give a higher bound.
-            const int k = p.n_top, k_part = min(k, part.n);
-            const bool nan = !(s == s);
-            float over = unordered(max(bound_of(ordered(mine), k, z.bound), ordered(-INFINITY)));
-            int n;
-            for (;;) {
-                __syncthreads();
-                if (threadIdx.x == 0) z.count = 0;
-                __syncthreads();
-                auto look = [&](float v, int at) {
-                    if (v > over) {
-                        const int i = atomicAdd(&z.count, 1);
-                        if (i < kCandidates) z.list[i] = candidate(v, c0 + at);
-                    }
-                };
-                if (!nan) {
-                    part.each_quad([&](int i, float4 v) {
-                        if (fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) > over) {
-                            const int at = part.head + 4 * i;
-                            look(v.x, at); look(v.y, at + 1); look(v.z, at + 2); look(v.w, at + 3);
-                        }
-                    });
-                    part.each_loose([&](int at, float v) { look(v, at); });
+            const size_t at = row * (size_t)k;
+            if (!(s == s)) {
+                if ((int)threadIdx.x < k) {
+                    if (p.top_ids != nullptr) p.top_ids[at + threadIdx.x] = -1;
+                    if (p.top_logprobs != nullptr) p.top_logprobs[at + threadIdx.x] = s;
                 }
-                __syncthreads();
-                n = z.count;
-                if (n <= kCandidates) break;
-                select_best(z, kCandidates, k);
-                over = unordered((uint32_t)(z.best[k - 1] >> 32));
+                continue;
             }
-            if (!nan && n < k_part) {                               // the lowest places of those equal to the bound
-                for (int c = 0; c < part.n && n < k_part; c += kRowThreads) {
-                    const int at = c + threadIdx.x;
-                    const float v = at < part.n ? load_behind(part.p + at) : 0.0f;
-                    const bool hit = at < part.n && v == over;
-                    const unsigned hits = __ballot_sync(0xffffffffu, hit);
-                    if (lane == 0) z.scanned[warp] = __popc(hits);
-                    __syncthreads();
-                    int before = n, all = n;
-                    for (int w = 0; w < kRowWarps; ++w) { if (w < warp) before += z.scanned[w]; all += z.scanned[w]; }
-                    before += __popc(hits & ((1u << lane) - 1));
-                    if (hit && before < k_part) z.list[before] = candidate(v, c0 + at);
-                    n = min(all, k_part);
-                    __syncthreads();
-                }
-            }
-            if (!nan) select_best(z, n, k_part);
-            if (ranks > 1) {
-                // the parts' lists are the candidates of the first CTA, which is behind its own selection when all have arrived
-                cluster_arrive();
-                cluster_wait();
-                if ((int)threadIdx.x < k && !nan) {
-                    const unsigned long long v = (int)threadIdx.x < k_part ? z.best[threadIdx.x] : 0ull;
-                    asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(cluster_address(&z.list[rank * k + threadIdx.x], 0)), "l"(v) : "memory");
-                }
-                cluster_arrive();
-                cluster_wait();
-                // empty places (0) of parts shorter than k are below every candidate; they fall out by rank since cols >= k
-                if (rank == 0 && !nan) {
-                    if ((int)threadIdx.x < ranks * k && z.list[threadIdx.x] == 0ull) z.list[threadIdx.x] = threadIdx.x;
-                    for (int i = threadIdx.x + kRowThreads; i < ranks * k; i += kRowThreads)
-                        if (z.list[i] == 0ull) z.list[i] = i;        // unlike one another
-                    __syncthreads();
-                    select_best(z, ranks * k, k);
-                }
-            }
-            if (rank == 0 && (int)threadIdx.x < k) {
-                const unsigned long long v = nan ? 0ull : z.best[threadIdx.x];
-                if (p.top_ids != nullptr) p.top_ids[row * k + threadIdx.x] = nan ? -1 : (int)(0xffffffffu - (uint32_t)v);
-                if (p.top_logprobs != nullptr) p.top_logprobs[row * k + threadIdx.x] = nan ? s : log_prob(unordered((uint32_t)(v >> 32)));
-            }
-            __syncthreads();
+            auto put = [&](int r, unsigned long long c) {
+                if (p.top_ids != nullptr) p.top_ids[at + r] = (int)(0xffffffffu - (uint32_t)c);
+                if (p.top_logprobs != nullptr) p.top_logprobs[at + r] = log_prob(unordered((uint32_t)(c >> 32)));
+            };
+            if (ranks == 1) each_best(z.list, n, k, put);
+            else each_best(gathered, ranks * k, k, put);
         }
-        if (DISTILL) {
-            const float t_sum = sh.t_sum;
-            if (warp == 0 && rank == 0 && p.losses != nullptr) {
-                float loss = 0.0f;
-                for (int i = lane; i < p.n_teacher; i += 32) {
-                    const float t = sh.t[i];
-                    if (t != 0.0f) loss += t * (sh.log_t[i] - log_prob(sh.x[i]));
-                }
-                loss = warp_add(loss);
-                if (lane == 0) p.losses[row] = loss;
-            }
-            if (p.grad_logits != nullptr) {
-                float* g = p.grad_logits + row * p.stride + c0;
-                const float up = load_behind(p.grad_out) * p.inv_t / (float)p.rows;
-                // an empty list or an empty row has no gradient; a list that is not a number has none that is one
-                const bool none = t_sum == 0.0f || s == 0.0f;
-                const float f = t_sum == t_sum ? up / s : t_sum;
-                auto value = [&](float v) { return exp2_fast(clamp_low((v - m) * p.c)) * f; };
-                if (none) clear_part(g, cn);
-                else write_part(part, g, value);
-                __syncthreads();
-                if (!none) write_listed(sh, p.n_teacher, g, c0, cn, up, value);
-            }
+        if (GRAD) {
+            const float sg = gradient_sum(s, list_warp.of(item).sum);
+            gm = m;
+            gf = up / sg;
+            none = sg == 0.0f;
         }
-        if (ranks > 1 && row + gridDim.x / ranks < p.rows) { cluster_arrive(); cluster_wait(); }
-        __syncthreads();                                            // what the CTA shares is another row's from here on
+        if (of_lists) {
+            const TeacherList& list = list_warp.of(item);
+            const float loss = list_loss(list, p.n_teacher, log_prob);
+            if (rank == 0) list_result(p, list, row, m, s, loss);
+            list_warp.ahead(item);
+        } else if (GRAD) write_part<THREADS>(part, q, p.grad_logits + row * p.stride + c0, again, loose, value);
+    }
+    if (GRAD) {
+        __syncthreads();
+        if (of_lists) write_behind(mine - 1);
+    }
+}
+
+// ---- loss and gradient of long rows in one pass ---------------------------------------------------------------------------
+// A row comes to shared memory once, in chunks by bulk copies, becomes its gradient there, and goes out by bulk copies: a ring of chunks in which the
+// next row comes while this one is at work and the one before goes.  The threads themselves neither load nor store: behind their own stores all
+// of an SM's memory instructions, those on shared memory among them, waited two thirds of the time (the row a second time out of L2: 300 us for 4096 x
+// 32000 with four rows on an SM, which L2 does not hold, 400 with two).
+// Two more warps: one has the teacher's lists and forms the losses; one issues the copies and writes the listed tokens' gradients a row behind.
+constexpr int kRingThreads = 512;      // that work on rows
+constexpr int kRingWarps = kRingThreads / 32;
+constexpr int kChunkQuads = 2 * kRingThreads;
+constexpr int kRingChunks = 13;
+// Chunks of a row.  At most: the last of a row is loaded when the one kRingChunks - 2 before it has left, which has to be of the row before.  At least: when a row's
+// statistics are there, its last chunk is, so the copying warp is at work on the row before or this one, and lists and statistics of three rows before are free.
+constexpr int kRingMost = kRingChunks - 2;
+constexpr int kRingLeast = 7;
+constexpr int kRingLists = 5;
+constexpr size_t kRingBytes = (size_t)kRingChunks * kChunkQuads * sizeof(float4);
+constexpr int kRingErr = 61;
+__device__ __forceinline__ void bulk_load(uint32_t to, const void* from, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(to), "l"(from), "r"(bytes), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void bulk_store(void* to, uint32_t from, uint32_t bytes) {
+    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(to), "r"(from), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void bulk_end() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+__global__ void __launch_bounds__(kRingThreads + 64, 1) distill_ring_kernel(VocabRows p, int chunks) {
+    grid_release();
+    extern __shared__ __align__(16) unsigned char dynamic[];
+    float4* ring = reinterpret_cast<float4*>(dynamic);
+    __shared__ float wm[2][kRingWarps], ws[2][kRingWarps], stat_m[4], stat_f[4];
+    __shared__ TeacherList lists[kRingLists];
+    __shared__ __align__(8) unsigned long long full[kRingChunks], done[kRingChunks];
+    __shared__ int gave_up;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const size_t mine = (p.rows - blockIdx.x + gridDim.x - 1) / gridDim.x;
+    if (threadIdx.x == 0) {
+        gave_up = 0;
+        for (int b = 0; b < kRingChunks; ++b) { mbar_init(smem_u32(&full[b]), 1); mbar_init(smem_u32(&done[b]), kRingWarps); }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+    grid_wait();
+    auto row_of = [&](size_t i) { return blockIdx.x + i * gridDim.x; };
+    auto part_of = [&](size_t i) { return Part(p.logits + row_of(i) * p.stride, p.cols); };
+    ListWarp<kRingLists, VocabRows, decltype(row_of)> list_warp = {lists, p, mine, row_of};
+    const float up = load_behind(p.grad_out) * p.inv_t / (float)p.rows;
+    // Where a wait runs out the call's results are void: the error word says so, nobody waits any more, and every loop runs to its end.
+    auto gone = [&] {
+        if (lane == 0) {
+            gave_up = 1;
+            *p.err_word = kRingErr;
+        }
+        __syncwarp();
+    };
+    if (warp == kRingWarps + 1) {
+        auto bytes_of = [&](const Part& part, int c) { return (uint32_t)max(0, min(kChunkQuads, part.n4 - c * kChunkQuads)) * 16u; };
+        const size_t stages = mine * chunks;
+        size_t ahead = 0;                                         // next stage to load, chunk ahead_c of item ahead_item
+        size_t ahead_item = 0;
+        int ahead_c = 0, slot_in = 0, slot_out = 0;
+        auto load = [&] {                                         // one lane
+            if (ahead >= stages) return;
+            const Part part = part_of(ahead_item);
+            const uint32_t n = bytes_of(part, ahead_c), bar = smem_u32(&full[slot_in]);
+            mbar_expect_tx(bar, n);
+            if (n > 0) bulk_load(smem_u32(ring + slot_in * kChunkQuads), part.quads() + ahead_c * kChunkQuads, n, bar);
+            ++ahead;
+            if (++ahead_c == chunks) { ahead_c = 0; ++ahead_item; }
+            if (++slot_in == kRingChunks) slot_in = 0;
+        };
+        if (lane == 0)
+            for (int i = 0; i < kRingChunks; ++i) load();
+        __syncwarp();
+        uint32_t parity = 0;
+        bool ok = true;
+        auto write_behind = [&](size_t item) {
+            const float m = stat_m[item & 3], f = stat_f[item & 3];
+            if (f != 0.0f)
+                list_write(list_warp.of(item), p.n_teacher, p.grad_logits + row_of(item) * p.stride, 0, p.cols, up,
+                           [&](float v) { return exp2_fast(clamp_low((v - m) * p.c)) * f; });
+        };
+        for (size_t item = 0; item < mine; ++item) {
+            const Part part = part_of(item);
+            float* g = p.grad_logits + row_of(item) * p.stride + part.head;
+#pragma unroll 1
+            for (int c = 0; c < chunks; ++c) {
+                if (ok && !mbar_wait_warp(smem_u32(&done[slot_out]), parity, &gave_up)) { ok = false; gone(); }
+                if (lane == 0 && ok) {
+                    const uint32_t n = bytes_of(part, c);
+                    if (n > 0) bulk_store(g + 4 * c * kChunkQuads, smem_u32(ring + slot_out * kChunkQuads), n);
+                    bulk_end();
+                    asm volatile("cp.async.bulk.wait_group.read 2;" ::: "memory");
+                    if (item > 0 || c >= 2) load();               // to where the chunk before the last two has left
+                }
+                if (++slot_out == kRingChunks) { slot_out = 0; parity ^= 1u; }
+            }
+            static_assert(kRingLeast >= 7, "what is pending is of this row");
+            if (lane == 0) asm volatile("cp.async.bulk.wait_group 7;" ::: "memory");
+            __syncwarp();
+            if (item > 0) write_behind(item - 1);
+        }
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+        __syncwarp();
+        write_behind(mine - 1);
+        return;
+    }
+    const bool of_lists = warp == kRingWarps;
+    if (of_lists) list_warp.start();
+    int slot = 0;                                                 // of this row's first chunk
+    uint32_t parity = 0;
+    bool ok = true;
+    for (size_t item = 0; item < mine; ++item) {
+        const size_t row = row_of(item);
+        const int turn = (int)(item & 1);
+        const Part part = part_of(item);
+        const bool has_loose = (int)threadIdx.x < part.n - 4 * part.n4;
+        const float loose = has_loose ? load_behind(part.p + part.loose(threadIdx.x)) : -INFINITY;
+        Stats<false> st;
+        int at_slot = slot;
+        uint32_t at_parity = parity;
+        if (!of_lists) {
+#pragma unroll 1
+            for (int c = 0; c < chunks; ++c) {
+                if (ok && !mbar_wait_warp(smem_u32(&full[at_slot]), at_parity, &gave_up)) { ok = false; gone(); }
+                float4 v[2];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const int i = u * kRingThreads + (int)threadIdx.x;
+                    v[u] = c * kChunkQuads + i < part.n4 ? ring[at_slot * kChunkQuads + i] : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+                }
+                const float top = fmaxf(top_of(v[0]), top_of(v[1]));
+                if (top > st.m) st.raise(top, p.c);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) { st.term(v[u].x, p.c); st.term(v[u].y, p.c); st.term(v[u].z, p.c); st.term(v[u].w, p.c); }
+                if (++at_slot == kRingChunks) { at_slot = 0; at_parity ^= 1u; }
+            }
+            st.add(loose, p.c);
+            st.join<32>(p.c);
+            if (lane == 0) { wm[turn][warp] = st.m; ws[turn][warp] = st.s; }
+        }
+        if (of_lists) list_warp.arrived();                        // before anything of this row may become its gradient (grad_logits == logits)
+        asm volatile("bar.sync 1, %0;" ::"n"(kRingThreads + 32) : "memory");
+        st.m = wm[turn][lane & (kRingWarps - 1)];
+        st.s = ws[turn][lane & (kRingWarps - 1)];
+        st.join<kRingWarps>(p.c);
+        // an empty list or an empty row has no gradient; a list that is not a number has none that is one
+        const TeacherList& list = list_warp.of(item);
+        const float m = st.m, s = st.s, sg = gradient_sum(s, list.sum), f = sg == 0.0f ? 0.0f : up / sg;
+        if (of_lists) {
+            const float log_s = logf(s);
+            const float loss = list_loss(list, p.n_teacher, [&](float v) { return s == 0.0f ? -INFINITY : (v - m) * p.inv_t - log_s; });
+            list_result(p, list, row, m, s, loss);
+            list_warp.ahead(item);
+            continue;
+        }
+        if (threadIdx.x == 0) { stat_m[item & 3] = m; stat_f[item & 3] = f; }
+        auto value = [&](float v) { return f == 0.0f ? 0.0f : exp2_fast(clamp_low((v - m) * p.c)) * f; };
+        if (has_loose) p.grad_logits[row * p.stride + part.loose(threadIdx.x)] = value(loose);
+#pragma unroll 1
+        for (int c = 0; c < chunks; ++c) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int i = u * kRingThreads + (int)threadIdx.x;
+                if (c * kChunkQuads + i >= part.n4) continue;
+                float4& at = ring[slot * kChunkQuads + i];
+                const float4 v = at;
+                at = make_float4(value(v.x), value(v.y), value(v.z), value(v.w));
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&done[slot])) : "memory");
+            if (++slot == kRingChunks) { slot = 0; parity ^= 1u; }
+        }
     }
 }
 
@@ -446,63 +925,71 @@ struct VocabGrad {
 };
 
 // dx_c = e_c (k0 + k1 d_c) + (what the named tokens add), with e_c = 2^((x_c - m) c): p_c enters through 1 / s in k0 and k1.
+// DISTILL: the first warp has an item's list on its way from the start, and takes the listed tokens' probabilities off when the rest is written.
 template <bool DISTILL>
-__global__ void __launch_bounds__(kRowThreads) vocab_grad_kernel(VocabGrad p) {
+__global__ void __launch_bounds__(kRowThreads, 4) vocab_grad_kernel(VocabGrad p) {
     grid_release();
     grid_wait();
-    __shared__ RowShared sh;
+    __shared__ TeacherList list;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const size_t items = p.rows * (size_t)p.tiles;
+    const int q = quarter_of(p.per, kRowThreads);
     for (size_t item = blockIdx.x; item < items; item += gridDim.x) {
         const size_t row = item / p.tiles;
-        const int c0 = (int)(item - row * p.tiles) * p.per, cn = min(p.cols, c0 + p.per) - c0;
+        const int c0 = (int)(item - row * p.tiles) * p.per, cn = min(p.cols - c0, p.per);
         const float* x = p.logits + row * p.stride;
         const Part part(x + c0, cn);
         float* g = p.grad_logits + row * p.stride + c0;
+        float4 v[kQuads];
+        load_step(part, q, 0, v);
+        const float loose = (int)threadIdx.x < part.n - 4 * part.n4 ? load_behind(part.p + part.loose(threadIdx.x)) : 0.0f;
         const float m = load_behind(p.row_stats + 2 * row), s = load_behind(p.row_stats + 2 * row + 1);
         float k0 = 0.0f, k1 = 0.0f, up = 0.0f, x_token = 0.0f;
         int token = -1;
-        bool none;
+        bool none = s == 0.0f;
         if (DISTILL) {
-            VocabRows list = {};
-            list.logits = p.logits; list.stride = p.stride; list.cols = p.cols; list.c = p.c;
-            list.teacher_ids = p.teacher_ids; list.teacher_logits = p.teacher_logits; list.n_teacher = p.n_teacher;
-            if (threadIdx.x < 32) read_list(list, row, sh);
-            __syncthreads();
+            if (warp == 0) { list_fetch(list, p, row); copies_end(); }
             up = load_behind(p.grad_out) * p.inv_t / (float)p.rows;
-            none = sh.t_sum == 0.0f;
-            k0 = sh.t_sum == sh.t_sum ? up / s : sh.t_sum;
+            k0 = up / s;
         } else {
             float h = 0.0f, H = 0.0f;
             if (p.grad_logprobs != nullptr) {
                 token = load_behind(p.tokens + row);
                 if (token < 0 || token >= p.cols) token = -1;
-                else { up = load_behind(p.grad_logprobs + row) * p.inv_t; x_token = load_behind(x + token); }
+                else {
+                    up = load_behind(p.grad_logprobs + row) * p.inv_t;
+                    if (threadIdx.x == 0) x_token = load_behind(x + token);
+                }
             }
             if (p.grad_entropy != nullptr) { h = load_behind(p.grad_entropy + row) * p.inv_t; H = load_behind(p.entropy + row); }
-            none = up == 0.0f && h == 0.0f;
+            none = none || (up == 0.0f && h == 0.0f);
             k0 = -(up + (h == 0.0f ? 0.0f : h * (H - logf(s)))) / s;
             k1 = -h * kLn2 / s;
-            __syncthreads();                                        // x_token is read before it may be overwritten (grad_logits == logits)
+            __syncthreads();        // the token's logit is read before any of the row is written (grad_logits may be logits); other tiles' are not used
         }
-        none = none || s == 0.0f;
-        auto value = [&](float v) {
-            const float d = clamp_low((v - m) * p.c);
-            return exp2_fast(d) * (DISTILL ? k0 : fmaf(k1, d, k0));
+        auto value = [&](float at) {
+            const float d = clamp_low((at - m) * p.c);
+            return none ? 0.0f : exp2_fast(d) * (DISTILL ? k0 : fmaf(k1, d, k0));
         };
-        if (none) clear_part(g, cn);
-        else write_part(part, g, value);
+        write_part<kRowThreads>(part, q, g, v, loose, value);
         __syncthreads();
-        if (!none && DISTILL) write_listed(sh, p.n_teacher, g, c0, cn, up, value);
-        if (!none && !DISTILL && threadIdx.x == 0 && token >= c0 && token < c0 + cn) g[token - c0] = value(x_token) + up;
-        if (DISTILL) __syncthreads();                               // the list is another item's from here on
+        if (!DISTILL && threadIdx.x == 0 && !none && token >= c0 && token < c0 + cn) g[token - c0] = value(x_token) + up;
+        if (DISTILL && warp == 0 && !none) {
+            copies_wait<0>();
+            __syncwarp();
+            for (int i = lane; i < p.n_teacher; i += 32)
+                if (list.id[i] < 0 || list.id[i] >= p.cols) list.t[i] = -INFINITY;
+            list_terms(list, p);
+            list_take_off(list, p.n_teacher, up, [&](int i) -> float* { return list.id[i] >= c0 && list.id[i] - c0 < cn ? g + (list.id[i] - c0) : nullptr; });
+        }
     }
 }
 
 // Attributes of a launch: overlapping with the one before it, and the CTAs of a row as a cluster.
 template <class P>
-cudaError_t launch_rows(void (*kern)(P), unsigned grid, int cluster, size_t smem, cudaStream_t stream, const P& p) {
+cudaError_t launch_rows(void (*kern)(P), unsigned grid, int threads, int cluster, size_t smem, cudaStream_t stream, const P& p) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid); cfg.blockDim = dim3(kRowThreads); cfg.dynamicSmemBytes = smem; cfg.stream = stream;
+    cfg.gridDim = dim3(grid); cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = smem; cfg.stream = stream;
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
@@ -517,9 +1004,29 @@ int row_cluster(size_t rows, int cols, int sm_count) {
     while (n < kMaxCluster && rows * 2 * n <= 2 * (size_t)sm_count && cols / (2 * n) >= 2048) n *= 2;
     return n;
 }
-unsigned row_ctas(size_t rows, int cluster, int sm_count) {
-    const size_t cap = (size_t)sm_count * 16 / cluster;
-    return (unsigned)((rows < cap ? rows : cap) * cluster);
+cudaError_t launch_forward(VocabRows& p, int sm_count, cudaStream_t stream) {
+    p.cluster = row_cluster(p.rows, p.cols, sm_count);
+    const size_t cap = (size_t)sm_count * 4;
+    const unsigned grid = p.cluster > 1 ? (unsigned)(p.rows * p.cluster) : (unsigned)(p.rows < cap ? p.rows : cap);
+    const bool distill = p.n_teacher > 0;
+    const size_t smem = kStreamBytes + (distill ? 3 * sizeof(TeacherList) : p.n_top ? sizeof(Selection) + (p.cluster > 1 ? kMaxCluster * kMaxList * sizeof(unsigned long long) : 0) : 0);
+    const auto kern = distill ? (p.grad_logits ? vocab_rows_kernel<false, kGrad> : vocab_rows_kernel<false, kList>)
+                    : p.n_top ? (p.entropy ? vocab_rows_kernel<true, kTop> : vocab_rows_kernel<false, kTop>)
+                              : (p.entropy ? vocab_rows_kernel<true, kPlain> : vocab_rows_kernel<false, kPlain>);
+    const cudaError_t e = smem <= 48 * 1024 - sizeof(RowShared) ? cudaSuccess : cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    return e != cudaSuccess ? e : launch_rows(kern, grid, kRowThreads, p.cluster, smem, stream, p);
+}
+// Rows of kRingLeast to kRingMost chunks, as many as keep all SMs busy, gradients on the logits' 16-byte boundaries.
+bool ring_takes(const VocabRows& p, int sm_count, size_t max_smem) {
+    const size_t chunks = ((size_t)(p.cols >> 2) + kChunkQuads - 1) / kChunkQuads;
+    return chunks >= kRingLeast && chunks <= kRingMost && p.rows >= 2 * (size_t)sm_count && kRingBytes + kRingLists * sizeof(TeacherList) + 1024 <= max_smem &&
+           ((reinterpret_cast<uintptr_t>(p.logits) ^ reinterpret_cast<uintptr_t>(p.grad_logits)) & 15) == 0;
+}
+cudaError_t launch_ring(VocabRows& p, int sm_count, cudaStream_t stream) {
+    const int chunks = ((p.cols >> 2) + kChunkQuads - 1) / kChunkQuads;
+    const cudaError_t e = cudaFuncSetAttribute(distill_ring_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kRingBytes);
+    if (e != cudaSuccess) return e;
+    return launch_chained(distill_ring_kernel, dim3((unsigned)(p.rows < (size_t)sm_count ? p.rows : sm_count)), dim3(kRingThreads + 64), kRingBytes, stream, p, chunks);
 }
 void temperature_of(float t, float* c, float* inv_t) {
     *inv_t = 1.0f / t;
@@ -533,7 +1040,7 @@ cudaError_t launch_grad(bool distill, VocabGrad& p, int sm_count, cudaStream_t s
     p.per = ((p.cols + p.tiles - 1) / p.tiles + 3) & ~3;
     p.tiles = (p.cols + p.per - 1) / p.per;
     const size_t items = p.rows * (size_t)p.tiles, cap = (size_t)sm_count * 16;
-    return launch_rows(distill ? vocab_grad_kernel<true> : vocab_grad_kernel<false>, (unsigned)(items < cap ? items : cap), 1, 0, stream, p);
+    return launch_rows(distill ? vocab_grad_kernel<true> : vocab_grad_kernel<false>, (unsigned)(items < cap ? items : cap), kRowThreads, 1, 0, stream, p);
 }
 }  // namespace
 
@@ -545,11 +1052,7 @@ cudaError_t launch_token_logprobs(const float* logits, const int* tokens, float*
     temperature_of(temperature, &p.c, &p.inv_t);
     p.tokens = tokens; p.logprobs = logprobs; p.entropy = entropy; p.top_ids = top_ids; p.top_logprobs = top_logprobs; p.n_top = n_top;
     p.row_stats = row_stats;
-    p.cluster = row_cluster(rows, cols, sm_count);
-    const unsigned grid = row_ctas(rows, p.cluster, sm_count);
-    const size_t smem = n_top ? sizeof(Selection) : 0;
-    if (n_top) return launch_rows(entropy ? vocab_rows_kernel<true, true, false> : vocab_rows_kernel<false, true, false>, grid, p.cluster, smem, stream, p);
-    return launch_rows(entropy ? vocab_rows_kernel<true, false, false> : vocab_rows_kernel<false, false, false>, grid, p.cluster, smem, stream, p);
+    return launch_forward(p, sm_count, stream);
 }
 cudaError_t launch_token_logprobs_backward(const float* logits, const int* tokens, const float* row_stats, const float* entropy,
                                            const float* grad_logprobs, const float* grad_entropy, float* grad_logits, size_t rows, int cols,
@@ -563,14 +1066,14 @@ cudaError_t launch_token_logprobs_backward(const float* logits, const int* token
 }
 cudaError_t launch_distillation_loss(const float* logits, const int* teacher_ids, const float* teacher_logits, float* losses, float* out,
                                      float* row_stats, const float* grad_out, float* grad_logits, size_t rows, int cols, size_t stride,
-                                     int n_teacher, float temperature, int sm_count, cudaStream_t stream) {
+                                     int n_teacher, float temperature, int* err_word, int sm_count, size_t max_smem, cudaStream_t stream) {
     VocabRows p = {};
     p.logits = logits; p.rows = rows; p.stride = stride; p.cols = cols;
     temperature_of(temperature, &p.c, &p.inv_t);
     p.teacher_ids = teacher_ids; p.teacher_logits = teacher_logits; p.n_teacher = n_teacher;
     p.losses = losses; p.row_stats = row_stats; p.grad_out = grad_out; p.grad_logits = grad_logits;
-    p.cluster = row_cluster(rows, cols, sm_count);
-    const cudaError_t e = launch_rows(vocab_rows_kernel<false, false, true>, row_ctas(rows, p.cluster, sm_count), p.cluster, 0, stream, p);
+    p.err_word = err_word;
+    const cudaError_t e = grad_logits != nullptr && ring_takes(p, sm_count, max_smem) ? launch_ring(p, sm_count, stream) : launch_forward(p, sm_count, stream);
     return e != cudaSuccess ? e : launch_mean(losses, out, rows, rows, stream);
 }
 cudaError_t launch_distillation_loss_backward(const float* logits, const int* teacher_ids, const float* teacher_logits, const float* row_stats,

@@ -397,7 +397,8 @@ FORMS = ["one call", "split", "in place", "split in place"]
 
 
 @pytest.mark.parametrize("R,V,K,pad,offset,T", [(1, 1, 1, 0, 0, 1.0), (3, 5, 5, 1, 1, 2.0), (20, 128, 128, 0, 0, 1.0), (33, 1001, 7, 0, 2, 0.5), (600, 2500, 64, 0, 0, 2.0),
-                                              (2500, 300, 3, 1, 0, 1.0), (1, 32000, 20, 0, 0, 1.0), (12, 33001, 128, 3, 1, 1.5), (40, 32000, 64, 0, 0, 4.0)])
+                                              (2500, 300, 3, 1, 0, 1.0), (1, 32000, 20, 0, 0, 1.0), (12, 33001, 128, 3, 1, 1.5), (40, 32000, 64, 0, 0, 4.0),
+                                              (300, 24581, 5, 0, 0, 1.0), (450, 32000, 64, 0, 0, 2.0), (310, 33001, 33, 3, 1, 0.7), (297, 45056, 128, 4, 3, 1.0)])
 @pytest.mark.parametrize("form", FORMS)
 def test_distillation(ctx, R, V, K, pad, offset, T, form):
     x, stride = make_logits(R, V, pad, offset, seed=10)
@@ -414,9 +415,9 @@ def test_distillation(ctx, R, V, K, pad, offset, T, form):
 
 
 @pytest.mark.parametrize("form", FORMS)
-@pytest.mark.parametrize("V", [500, 40000])
-def test_distillation_lists_and_rows_that_go_wrong(ctx, V, form):
-    R, K = 16, 10
+@pytest.mark.parametrize("R,V", [(16, 500), (16, 40000), (320, 26000)])
+def test_distillation_lists_and_rows_that_go_wrong(ctx, R, V, form):
+    K = 10
     x, stride = make_logits(R, V, 1, 0, seed=11)
     special_rows(x)
     ids, a = make_teacher(R, V, K, 2)
@@ -438,9 +439,35 @@ def test_distillation_lists_and_rows_that_go_wrong(ctx, V, form):
     assert float(part[0]) == math.inf and float(part[11]) == 0.0
 
 
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("K", [33, 64, 128])
+def test_distillation_lists_longer_than_a_warp(ctx, K, form):
+    """Entries without a token and tokens named twice, in every group of 32 entries and across them."""
+    R, V = 12, 3000
+    x, stride = make_logits(R, V, 1, 0, seed=16)
+    ids, a = make_teacher(R, V, K, 5)
+    ids[0] = -1
+    ids[1, 0] = -1
+    ids[2, ::2] = -1
+    ids[3, 31], ids[3, 32] = -1, -32                                # any number outside the vocabulary
+    ids[4, K - 1] = ids[4, 0]
+    ids[5, 32] = ids[5, 1]
+    ids[6] = torch.arange(K) % 7
+    ids[7, 1] = ids[7, 0]
+    ids[8, K - 1] = ids[8, K - 2]
+    ids[9] = V + torch.arange(K)
+    ids[9, K - 1] = 3
+    ids[10, :32] = -1
+    losses, tol_l, grad, tol_g = distill_ref(x, ids, a, 1.25)
+    part, out, got = run_distill(ctx, x, stride, ids, a, 1.25, 1.0, form)
+    near(part, losses, tol_l, "losses")
+    near(got, grad, tol_g, "gradient")
+
+
 @pytest.mark.parametrize("form", ["one call", "split"])
-def test_distillation_of_rows_with_nan(ctx, form):
-    R, V, K = 7, 3000, 5
+@pytest.mark.parametrize("R,V", [(7, 3000), (300, 25001)])
+def test_distillation_of_rows_with_nan(ctx, R, V, form):
+    K = 5
     x, stride = make_logits(R, V, seed=12)
     ids, a = make_teacher(R, V, K, 3)
     x[0, 7] = math.nan
@@ -450,7 +477,7 @@ def test_distillation_of_rows_with_nan(ctx, form):
     a[3, 2] = math.nan
     a[4, 2] = math.inf
     part, out, got = run_distill(ctx, x, stride, ids, a, 1.0, 1.0, form)
-    bad = torch.tensor([True, True, False, True, True, False, False])
+    bad = torch.tensor([True, True, False, True, True] + [False] * (R - 5))
     assert torch.equal(torch.isnan(part).cpu(), bad) and torch.equal(torch.isnan(got).any(dim=1).cpu(), bad)
     assert torch.equal(torch.isnan(got).all(dim=1).cpu(), bad)
     assert float(part[2]) == 0.0 and bool((got[2] == 0.0).all())
