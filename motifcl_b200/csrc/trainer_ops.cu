@@ -216,7 +216,164 @@ __global__ void __launch_bounds__(256) rmsnorm_bwd_w_kernel(const float* x, cons
 // y = (x - mean) r w + b with r = 1 / sqrt(var + eps).  With n = (x - mean) r and g = dy w:
 //     dx = r (g - mean(g) - n mean(g n))      dw = sum of dy n over the rows      db = sum of dy
 // The variance is the mean of (x - mean)^2, not a difference of two sums, which a mean far from zero would leave no digits of.
-// A block per row; rows are read again from L1.
+// Up to 8192 columns: W warps per row, each lane J times four columns in registers, the next row's loads in flight while this one's sums are formed, so
+// that memory sees every tensor once.  VEC: 16-byte accesses (rows on 16-byte boundaries); else a lane's columns are W * 32 apart, so that a warp's
+// accesses are whole lines all the same.
+template <int W, int J, bool VEC>
+struct NormCols {
+    int t, cols;
+    __device__ __forceinline__ int at(int j, int i) const { return VEC ? 4 * (t + W * 32 * j) + i : t + W * 32 * (4 * j + i); }
+    __device__ __forceinline__ bool in(int j, int i) const { return at(j, VEC ? 0 : i) < cols; }
+    __device__ __forceinline__ void get(const float* r, float (&v)[4 * J]) const {       // 0 behind the row
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            if (VEC) {
+                const float4 f = in(j, 0) ? load_behind(reinterpret_cast<const float4*>(r + at(j, 0))) : make_float4(0.f, 0.f, 0.f, 0.f);
+                v[4 * j] = f.x; v[4 * j + 1] = f.y; v[4 * j + 2] = f.z; v[4 * j + 3] = f.w;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[4 * j + i] = in(j, i) ? load_behind(r + at(j, i)) : 0.0f;
+            }
+        }
+    }
+    __device__ __forceinline__ void put(float* r, const float (&v)[4 * J]) const {
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            if (VEC) {
+                if (in(j, 0)) *reinterpret_cast<float4*>(r + at(j, 0)) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (in(j, i)) r[at(j, i)] = v[4 * j + i];
+            }
+        }
+    }
+};
+template <int W>
+constexpr int kNormThreads = W <= 8 ? 256 : W * 32;
+// Sums over the W warps of a row; `red` alternates between two places from call to call, so that one barrier is enough.
+template <int W>
+__device__ __forceinline__ float2 row_sum(float2 v, float2 (*red)[32], int& turn) {
+    v.x = warp_sum(v.x);
+    v.y = warp_sum(v.y);
+    if (W == 1) return v;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if (lane == 0) red[turn][warp] = v;
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + warp / W), "n"(W * 32) : "memory");
+    v = red[turn][warp / W * W + (lane & (W - 1))];
+    turn ^= 1;
+#pragma unroll
+    for (int o = W / 2; o > 0; o >>= 1) { v.x += __shfl_xor_sync(0xffffffffu, v.x, o); v.y += __shfl_xor_sync(0xffffffffu, v.y, o); }
+    return v;
+}
+template <int W, int J, bool VEC>
+__global__ void __launch_bounds__(kNormThreads<W>) layernorm_rows_kernel(const float* x, const float* w, const float* b, float* out, float* row_stats,
+                                                                         size_t rows, int cols, float eps) {
+    constexpr int G = kNormThreads<W> / (W * 32);
+    grid_release();
+    __shared__ float2 red[2][32];
+    const NormCols<W, J, VEC> c = {(int)(threadIdx.x % (W * 32)), cols};
+    const size_t first = (size_t)blockIdx.x * G + threadIdx.x / (W * 32), step = (size_t)gridDim.x * G;
+    grid_wait();
+    float wv[4 * J], bv[4 * J], v[4 * J], next[4 * J];
+    c.get(w, wv);
+#pragma unroll
+    for (int i = 0; i < 4 * J; ++i) bv[i] = 0.0f;
+    if (b != nullptr) c.get(b, bv);
+    if (first < rows) c.get(x + first * cols, v);
+    int turn = 0;
+    for (size_t row = first; row < rows; row += step) {
+        if (row + step < rows) c.get(x + (row + step) * cols, next);
+        float sum = 0.0f, sq = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4 * J; ++i) sum += v[i];
+        const float mean = row_sum<W>(make_float2(sum, 0.0f), red, turn).x / (float)cols;
+#pragma unroll
+        for (int i = 0; i < 4 * J; ++i) {
+            v[i] -= mean;
+            if (c.in(i / 4, i % 4)) sq += v[i] * v[i];
+        }
+        const float inv = 1.0f / sqrtf(row_sum<W>(make_float2(sq, 0.0f), red, turn).x / (float)cols + eps);
+#pragma unroll
+        for (int i = 0; i < 4 * J; ++i) v[i] = v[i] * inv * wv[i] + bv[i];
+        c.put(out + row * cols, v);
+        if (row_stats != nullptr && c.t == 0) { row_stats[2 * row] = mean; row_stats[2 * row + 1] = inv; }
+#pragma unroll
+        for (int i = 0; i < 4 * J; ++i) v[i] = next[i];
+    }
+}
+// dx of a row, and the row's part of dw and db in the registers of those who have its columns; partial [CTAs][cols] of each at the end.
+template <int W, int J, bool VEC>
+__global__ void __launch_bounds__(kNormThreads<W>) layernorm_bwd_rows_kernel(const float* x, const float* w, const float* dy, const float* row_stats, float* dx,
+                                                                             float* dw_part, float* db_part, size_t rows, int cols) {
+    constexpr int G = kNormThreads<W> / (W * 32);
+    grid_release();
+    __shared__ float2 red[2][32];
+    __shared__ float part[4][kNormThreads<W>];
+    const NormCols<W, J, VEC> c = {(int)(threadIdx.x % (W * 32)), cols};
+    const size_t first = (size_t)blockIdx.x * G + threadIdx.x / (W * 32), step = (size_t)gridDim.x * G;
+    grid_wait();
+    float wv[4 * J], aw[4 * J], ab[4 * J], v[4 * J], g[4 * J], next_v[4 * J], next_g[4 * J];
+    float mean = 0.0f, inv = 0.0f, next_mean = 0.0f, next_inv = 0.0f;
+    c.get(w, wv);
+#pragma unroll
+    for (int i = 0; i < 4 * J; ++i) aw[i] = ab[i] = 0.0f;
+    auto fetch = [&](size_t row, float (&xv)[4 * J], float (&gv)[4 * J], float& m, float& r) {
+        c.get(x + row * cols, xv);
+        c.get(dy + row * cols, gv);
+        m = load_behind(row_stats + 2 * row);
+        r = load_behind(row_stats + 2 * row + 1);
+    };
+    if (first < rows) fetch(first, v, g, mean, inv);
+    int turn = 0;
+    for (size_t row = first; row < rows; row += step) {
+        if (row + step < rows) fetch(row + step, next_v, next_g, next_mean, next_inv);
+        float sg = 0.0f, sgn = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4 * J; ++i) {
+            v[i] = c.in(i / 4, i % 4) ? (v[i] - mean) * inv : 0.0f;
+            aw[i] += g[i] * v[i];
+            ab[i] += g[i];
+            g[i] *= wv[i];
+            sg += g[i];
+            sgn += g[i] * v[i];
+        }
+        if (dx != nullptr) {
+            const float2 sums = row_sum<W>(make_float2(sg, sgn), red, turn);
+            const float mg = sums.x / (float)cols, mgn = sums.y / (float)cols;
+#pragma unroll
+            for (int i = 0; i < 4 * J; ++i) g[i] = inv * (g[i] - mg - v[i] * mgn);
+            c.put(dx + row * cols, g);
+        }
+#pragma unroll
+        for (int i = 0; i < 4 * J; ++i) { v[i] = next_v[i]; g[i] = next_g[i]; }
+        mean = next_mean;
+        inv = next_inv;
+    }
+    // the groups of a CTA, then the CTA's part
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+        float* to = which == 0 ? dw_part : db_part;
+        if (to == nullptr) continue;
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) part[i][threadIdx.x] = which == 0 ? aw[4 * j + i] : ab[4 * j + i];
+            __syncthreads();
+            if (threadIdx.x < W * 32) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float s = 0.0f;
+#pragma unroll
+                    for (int k = 0; k < G; ++k) s += part[i][k * W * 32 + threadIdx.x];
+                    if (c.at(j, i) < cols) to[(size_t)blockIdx.x * cols + c.at(j, i)] = s;
+                }
+            }
+        }
+    }
+}
+// Longer rows: a block per row, which is read again from L1; columns in blocks of 32 for dw and db.
 __global__ void __launch_bounds__(256) layernorm_kernel(const float* x, const float* w, const float* b, float* out, float* row_stats, size_t rows,
                                                         Vec4 a, float eps) {
     grid_release();
@@ -297,10 +454,10 @@ __global__ void __launch_bounds__(256) layernorm_bwd_w_kernel(const float* x, co
     }
 }
 // out[c] = sum of part[i][c] over the splits, always in the same order; blockIdx.y: weight, bias
-__global__ void __launch_bounds__(256) layernorm_sum_kernel(const float* dw_part, const float* db_part, float* dw, float* db, int splits, int cols) {
+__global__ void __launch_bounds__(1024) layernorm_sum_kernel(const float* dw_part, const float* db_part, float* dw, float* db, int splits, int cols) {
     grid_release();
     grid_wait();
-    __shared__ float part[8][33];
+    __shared__ float part[32][33];
     const int cx = threadIdx.x & 31, ry = threadIdx.x >> 5;
     const int col = blockIdx.x * 32 + cx;
     const float* from = blockIdx.y == 0 ? dw_part : db_part;
@@ -308,15 +465,12 @@ __global__ void __launch_bounds__(256) layernorm_sum_kernel(const float* dw_part
     if (to == nullptr) return;
     float s = 0.0f;
     if (col < cols)
-        for (int i = ry; i < splits; i += 8) s += from[(size_t)i * cols + col];
+#pragma unroll 4
+        for (int i = ry; i < splits; i += 32) s += load_behind(from + (size_t)i * cols + col);
     part[ry][cx] = s;
     __syncthreads();
-    if (ry == 0 && col < cols) {
-        s = 0.0f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) s += part[j][cx];
-        to[col] = s;
-    }
+    s = warp_sum(part[cx][ry]);                     // a warp per column
+    if (cx == 0 && blockIdx.x * 32 + ry < cols) to[blockIdx.x * 32 + ry] = s;
 }
 
 // ---- swiglu ----------------------------------------------------------------------------------
@@ -823,14 +977,54 @@ cudaError_t launch_rmsnorm_backward_weight(const float* x, const float* dy, floa
     launch_chained(rmsnorm_bwd_w_kernel, dim3(col_blocks, (unsigned)splits), dim3(256), 0, stream, x, dy, row_inv, dw, rows, cols, rows_per_block);
     return cudaGetLastError();
 }
-cudaError_t launch_layernorm(const float* x, const float* w, const float* b, float* out, float* row_stats, size_t rows, int cols, float eps,
-                             int sm_count, cudaStream_t stream) {
-    const Vec4 a = {cols % 4 == 0 && all16(x, w, out, b), cols};
-    launch_chained(layernorm_kernel, dim3(row_grid(rows, sm_count)), dim3(256), 0, stream, x, w, b, out, row_stats, rows, a, eps);
-    return cudaGetLastError();
-}
 namespace {
+// f(kernel template arguments) by the columns: up to 512 a warp per row, above it eight columns a thread
+template <class F>
+cudaError_t norm_by_cols(int cols, bool vec, F f) {
+    if (cols <= 128) return vec ? f.template run<1, 1, true>() : f.template run<1, 1, false>();
+    if (cols <= 256) return vec ? f.template run<1, 2, true>() : f.template run<1, 2, false>();
+    if (cols <= 384) return vec ? f.template run<1, 3, true>() : f.template run<1, 3, false>();
+    if (cols <= 512) return vec ? f.template run<2, 2, true>() : f.template run<2, 2, false>();
+    if (cols <= 1024) return vec ? f.template run<4, 2, true>() : f.template run<4, 2, false>();
+    if (cols <= 2048) return vec ? f.template run<8, 2, true>() : f.template run<8, 2, false>();
+    if (cols <= 4096) return vec ? f.template run<16, 2, true>() : f.template run<16, 2, false>();
+    return vec ? f.template run<32, 2, true>() : f.template run<32, 2, false>();
+}
+constexpr int kNormCols = 8192;
+int norm_groups(int cols) { return cols <= 384 ? 8 : cols <= 512 ? 4 : cols <= 1024 ? 2 : 1; }       // rows of a CTA at a time
+struct NormForward {
+    const float *x, *w, *b;
+    float *out, *row_stats;
+    size_t rows;
+    int cols;
+    float eps;
+    int sm_count;
+    cudaStream_t stream;
+    template <int W, int J, bool VEC>
+    cudaError_t run() const {
+        const size_t want = (rows + norm_groups(cols) - 1) / norm_groups(cols), cap = (size_t)sm_count * (2048 / kNormThreads<W>);
+        return launch_chained(layernorm_rows_kernel<W, J, VEC>, dim3((unsigned)(want < cap ? want : cap)), dim3(kNormThreads<W>), 0, stream, x, w, b, out, row_stats, rows,
+                              cols, eps);
+    }
+};
+struct NormBackward {
+    const float *x, *w, *dy, *row_stats;
+    float *dx, *dw_part, *db_part;
+    size_t rows;
+    int cols;
+    unsigned grid;
+    cudaStream_t stream;
+    template <int W, int J, bool VEC>
+    cudaError_t run() const {
+        return launch_chained(layernorm_bwd_rows_kernel<W, J, VEC>, dim3(grid), dim3(kNormThreads<W>), 0, stream, x, w, dy, row_stats, dx, dw_part, db_part, rows, cols);
+    }
+};
+// CTAs of the backward pass, or row splits of the kernel for longer rows: parts that dw and db are added up from
 size_t layernorm_splits(size_t rows, int cols, int sm_count) {
+    if (cols <= kNormCols) {                          // four rows to a group at least: every CTA ends in a part of its own
+        const size_t per = 4 * (size_t)norm_groups(cols), want = (rows + per - 1) / per, cap = (size_t)sm_count * (cols <= 2048 ? 3 : cols <= 4096 ? 2 : 1);
+        return want < cap ? want : cap;
+    }
     const size_t col_blocks = ((size_t)cols + 31) / 32;
     size_t splits = ((size_t)sm_count * 8 + col_blocks - 1) / col_blocks;
     if (splits > (rows + 63) / 64) splits = (rows + 63) / 64;
@@ -838,25 +1032,38 @@ size_t layernorm_splits(size_t rows, int cols, int sm_count) {
     return (rows + per - 1) / per;
 }
 }  // namespace
+cudaError_t launch_layernorm(const float* x, const float* w, const float* b, float* out, float* row_stats, size_t rows, int cols, float eps,
+                             int sm_count, cudaStream_t stream) {
+    const bool vec = cols % 4 == 0 && all16(x, w, out, b);
+    if (cols <= kNormCols) return norm_by_cols(cols, vec, NormForward{x, w, b, out, row_stats, rows, cols, eps, sm_count, stream});
+    return launch_chained(layernorm_kernel, dim3(row_grid(rows, sm_count)), dim3(256), 0, stream, x, w, b, out, row_stats, rows, Vec4{vec, cols}, eps);
+}
 size_t layernorm_partial_floats(size_t rows, int cols, bool dw, bool db, int sm_count) {
     return (size_t)(dw + db) * layernorm_splits(rows, cols, sm_count) * (size_t)cols;
 }
 cudaError_t launch_layernorm_backward(const float* x, const float* w, const float* dy, const float* row_stats, float* dx, float* dw, float* db,
                                       float* partial, size_t rows, int cols, int sm_count, cudaStream_t stream, int* launches) {
     cudaError_t e;
-    if (dw != nullptr || db != nullptr) {           // first: dx may take the place of x or dy
-        const size_t splits = layernorm_splits(rows, cols, sm_count), per = (rows + splits - 1) / splits;
-        float* dw_part = dw != nullptr ? partial : nullptr;
-        float* db_part = db != nullptr ? partial + (dw != nullptr ? splits * (size_t)cols : 0) : nullptr;
-        const unsigned blocks = (unsigned)((cols + 31) / 32);
+    const bool sums = dw != nullptr || db != nullptr, vec = cols % 4 == 0 && all16(x, w, dy, dx);
+    const size_t splits = layernorm_splits(rows, cols, sm_count);
+    float* dw_part = dw != nullptr ? partial : nullptr;
+    float* db_part = db != nullptr ? partial + (dw != nullptr ? splits * (size_t)cols : 0) : nullptr;
+    const unsigned blocks = (unsigned)((cols + 31) / 32);
+    if (cols <= kNormCols) {
+        if ((e = norm_by_cols(cols, vec, NormBackward{x, w, dy, row_stats, dx, dw_part, db_part, rows, cols, (unsigned)splits, stream})) != cudaSuccess) return e;
+        *launches += 1;
+    } else if (sums) {                                // first: dx may take the place of x or dy
+        const size_t per = (rows + splits - 1) / splits;
         if ((e = launch_chained(layernorm_bwd_w_kernel, dim3(blocks, (unsigned)splits), dim3(256), 0, stream, x, dy, row_stats, dw_part, db_part, rows, cols, per)) != cudaSuccess) return e;
-        if ((e = launch_chained(layernorm_sum_kernel, dim3(blocks, 2), dim3(256), 0, stream, dw_part, db_part, dw, db, (int)splits, cols)) != cudaSuccess) return e;
-        *launches += 2;
+        *launches += 1;
     }
-    if (dx == nullptr) return cudaSuccess;
-    const Vec4 a = {cols % 4 == 0 && all16(x, w, dy, dx), cols};
+    if (sums) {
+        if ((e = launch_chained(layernorm_sum_kernel, dim3(blocks, 2), dim3(1024), 0, stream, dw_part, db_part, dw, db, (int)splits, cols)) != cudaSuccess) return e;
+        *launches += 1;
+    }
+    if (cols <= kNormCols || dx == nullptr) return cudaSuccess;
     *launches += 1;
-    return launch_chained(layernorm_bwd_x_kernel, dim3(row_grid(rows, sm_count)), dim3(256), 0, stream, x, w, dy, row_stats, dx, rows, a);
+    return launch_chained(layernorm_bwd_x_kernel, dim3(row_grid(rows, sm_count)), dim3(256), 0, stream, x, w, dy, row_stats, dx, rows, Vec4{vec, cols});
 }
 cudaError_t launch_mean(const float* in, float* out, size_t n, size_t denominator, cudaStream_t stream) {
     return launch_chained(mean_kernel, dim3(1), dim3(1024), 0, stream, in, out, n, denominator);
