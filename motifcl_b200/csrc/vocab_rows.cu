@@ -18,11 +18,12 @@ namespace {
 
 constexpr int kRowThreads = 256;
 constexpr int kRowWarps = kRowThreads / 32;
+constexpr int kResultThread = kRowThreads - 32;        // writes a row's results: the first of the warp that has least to do at the end
 constexpr int kQuads = 4;              // of a thread in flight
 constexpr int kMaxList = kVocabListMax;
 constexpr int kMaxCluster = 8;
-constexpr int kHits = 1024;            // quads with a value above a row's first bound
-constexpr int kCandidates = 1024;      // values that reach its last one
+constexpr int kHits = 768;             // quads with a value above a row's first bounds
+constexpr int kCandidates = 512;       // values that reach its last one
 constexpr float kLn2 = 0.69314718f;    // ln 2 to fp32
 
 // max(v, -150) that keeps NaN
@@ -47,6 +48,33 @@ __device__ __forceinline__ float warp_top(float v) {
     return v;
 }
 
+// Two fp32 values in one register pair: an instruction for both.
+typedef unsigned long long Pair;
+__device__ __forceinline__ Pair pair_of(float a, float b) {
+    Pair r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float low_of(Pair v) { return __uint_as_float((uint32_t)v); }
+__device__ __forceinline__ float high_of(Pair v) { return __uint_as_float((uint32_t)(v >> 32)); }
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+    Pair r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+    Pair r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+    Pair r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ Pair clamp2(Pair v) { return pair_of(clamp_low(low_of(v)), clamp_low(high_of(v))); }
+__device__ __forceinline__ Pair exp2_2(Pair v) { return pair_of(exp2_fast(low_of(v)), exp2_fast(high_of(v))); }
+
 // ---- running statistics of a part of a row -----------------------------------------------------------------------------
 // c = log2(e) / T.  m: largest so far (the lowest float where nothing was above it), s: sum of e = 2^((x - m) c), a: sum of e (x - m) c.
 template <bool ENTROPY>
@@ -57,15 +85,6 @@ struct Stats {
         if (ENTROPY) a = f * (a + d * s);
         s *= f;
         m = to;
-    }
-    __device__ __forceinline__ void term(float x, float c) {
-        const float d = clamp_low((x - m) * c), e = exp2_fast(d);
-        s += e;
-        if (ENTROPY) a = fmaf(e, d, a);
-    }
-    __device__ __forceinline__ void add(float x, float c) {
-        if (x > m) raise(x, c);
-        term(x, c);
     }
     // of the lanes xor 1 .. `lanes` / 2
     template <int LANES>
@@ -80,6 +99,44 @@ struct Stats {
             if (ENTROPY) a += __shfl_xor_sync(0xffffffffu, a, o);
         }
     }
+};
+// The same while values go by, in two sums each.  Where there is no a to form, nothing needs a clamp: 2^-infinity is 0.
+template <bool ENTROPY>
+struct Running {
+    float m = -FLT_MAX;
+    Pair minus_m = pair_of(FLT_MAX, FLT_MAX), s = 0, a = 0;
+    __device__ __forceinline__ void raise(float to, float c) {
+        const float d = clamp_low((m - to) * c), f = exp2_fast(d);
+        if (ENTROPY) a = mul2(fma2(pair_of(d, d), s, a), pair_of(f, f));
+        s = mul2(s, pair_of(f, f));
+        m = to;
+        minus_m = pair_of(-to, -to);
+    }
+    __device__ __forceinline__ void terms(Pair x, float c) {
+        Pair d = mul2(add2(x, minus_m), pair_of(c, c));
+        if (ENTROPY) d = clamp2(d);
+        const Pair e = exp2_2(d);
+        s = add2(s, e);
+        if (ENTROPY) a = fma2(e, d, a);
+    }
+    template <int N>
+    __device__ __forceinline__ void quads(const float4 (&v)[N], float top, float c) {      // top: the largest of them
+        if (top > m) raise(top, c);
+#pragma unroll
+        for (int u = 0; u < N; ++u) { terms(pair_of(v[u].x, v[u].y), c); terms(pair_of(v[u].z, v[u].w), c); }
+    }
+    __device__ __forceinline__ void one(float x, float c) {
+        if (x > m) raise(x, c);
+        terms(pair_of(x, -INFINITY), c);
+    }
+    __device__ __forceinline__ Stats<ENTROPY> sums() const {
+        Stats<ENTROPY> r;
+        r.m = m;
+        r.s = low_of(s) + high_of(s);
+        if (ENTROPY) r.a = low_of(a) + high_of(a);
+        return r;
+    }
+    __device__ __forceinline__ float largest() const { return m == -FLT_MAX ? -INFINITY : m; }       // of what has gone by: no more than that
 };
 __device__ __forceinline__ float top_of(float4 v) { return fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)); }
 
@@ -126,11 +183,13 @@ struct Stream {
     }
     __device__ __forceinline__ void fetch(int to) {
         if (next_item < items && q > 0) {
+            const int i = t + (int)threadIdx.x;
+            const float4* from = at.quads() + i;
+            float4* place = ring + to * kQuads * THREADS + threadIdx.x;
+            const bool whole = t + (kQuads - 1) * q + THREADS <= at.n4;
 #pragma unroll
-            for (int u = 0; u < kQuads; ++u) {
-                const int i = u * q + t + (int)threadIdx.x;
-                if (i < at.n4) copy_async16(ring + (to * kQuads + u) * THREADS + threadIdx.x, at.quads() + i);
-            }
+            for (int u = 0; u < kQuads; ++u)
+                if (whole || u * q + i < at.n4) copy_async16(place + u * THREADS, from + u * q);
             t += THREADS;
             if (t >= q) {
                 t = 0;
@@ -142,9 +201,13 @@ struct Stream {
     // step `now` of a part with n4 quads: -infinity behind the end.  next() follows when the values have been used
     __device__ __forceinline__ void take(int now, int n4, float4 (&v)[kQuads]) {
         copies_wait<kAhead - 1>();
+        const float4* place = ring + slot * kQuads * THREADS + threadIdx.x;
+#pragma unroll
+        for (int u = 0; u < kQuads; ++u) v[u] = place[u * THREADS];
+        if (now + (kQuads - 1) * q + THREADS <= n4) return;
 #pragma unroll
         for (int u = 0; u < kQuads; ++u)
-            v[u] = u * q + now + (int)threadIdx.x < n4 ? ring[(slot * kQuads + u) * THREADS + threadIdx.x] : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+            if (u * q + now + (int)threadIdx.x >= n4) v[u] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
     }
     __device__ __forceinline__ void next() {
         fetch(slot);
@@ -162,8 +225,30 @@ __device__ __forceinline__ void load_step(const Part& part, int q, int t, float4
         if (i < part.n4) v[u] = load_behind(part.quads() + i);
     }
 }
+// The gradients that f may be: f times p (1 / s is in f), and with the entropy's part e (k0 + k1 d).
+struct ProbGrad {
+    float m, c, f;
+    __device__ __forceinline__ Pair operator()(Pair x) const { return mul2(exp2_2(mul2(add2(x, pair_of(-m, -m)), pair_of(c, c))), pair_of(f, f)); }
+    __device__ __forceinline__ float operator()(float x) const { return exp2_fast((x - m) * c) * f; }
+};
+struct EntropyGrad {
+    float m, c, k0, k1;
+    __device__ __forceinline__ Pair operator()(Pair x) const {
+        const Pair d = clamp2(mul2(add2(x, pair_of(-m, -m)), pair_of(c, c)));
+        return mul2(exp2_2(d), fma2(pair_of(k1, k1), d, pair_of(k0, k0)));
+    }
+    __device__ __forceinline__ float operator()(float x) const {
+        const float d = clamp_low((x - m) * c);
+        return exp2_fast(d) * fmaf(k1, d, k0);
+    }
+};
+template <class F>
+__device__ __forceinline__ float4 quad_of(float4 v, F f) {
+    const Pair a = f(pair_of(v.x, v.y)), b = f(pair_of(v.z, v.w));
+    return make_float4(low_of(a), high_of(a), low_of(b), high_of(b));
+}
 template <int THREADS, class F>
-__device__ __forceinline__ void write_part(const Part& part, int q, float* g, float4 (&v)[kQuads], float loose, F f) {
+__device__ __forceinline__ void write_part(const Part& part, int q, float* g, float4 (&v)[kQuads], float loose, bool none, F f) {
     const bool vec = ((reinterpret_cast<uintptr_t>(g) ^ reinterpret_cast<uintptr_t>(part.p)) & 15) == 0;
     float4 next[kQuads];
 #pragma unroll 1
@@ -174,14 +259,14 @@ __device__ __forceinline__ void write_part(const Part& part, int q, float* g, fl
             const int i = u * q + t + (int)threadIdx.x;
             if (i >= part.n4) continue;
             float* to = g + part.head + 4 * i;
-            const float4 o = make_float4(f(v[u].x), f(v[u].y), f(v[u].z), f(v[u].w));
+            const float4 o = none ? make_float4(0.f, 0.f, 0.f, 0.f) : quad_of(v[u], f);
             if (vec) *reinterpret_cast<float4*>(to) = o;
             else { to[0] = o.x; to[1] = o.y; to[2] = o.z; to[3] = o.w; }
         }
 #pragma unroll
         for (int u = 0; u < kQuads; ++u) v[u] = next[u];
     }
-    if ((int)threadIdx.x < part.n - 4 * part.n4) g[part.loose(threadIdx.x)] = f(loose);
+    if ((int)threadIdx.x < part.n - 4 * part.n4) g[part.loose(threadIdx.x)] = none ? 0.0f : f(loose);
 }
 
 // ---- selection of the largest ------------------------------------------------------------------------------------------
@@ -197,7 +282,8 @@ __device__ __forceinline__ unsigned long long candidate(float v, int at) {
 struct Selection {
     unsigned long long list[kCandidates];
     unsigned long long best[kMaxList];     // largest first
-    int hits[kHits];                       // quads
+    float4 hit[kHits];                     // quads, and their numbers
+    int hit_at[kHits];
     uint32_t bound[2][kRowWarps];
     int n_hits[2], n_list[2], scanned[kRowWarps];
 };
@@ -245,12 +331,43 @@ __device__ __forceinline__ void each_best(const unsigned long long* list, int n,
         if (part == 0 && i < n && rank < k) f(rank, v);
     }
 }
-// To list: the values of v, a quad at `at`, that reach `least`, or are above it (strict).
-__device__ __forceinline__ void take(Selection& z, int* count, float v, int at, float least, bool strict) {
-    if (!(v >= least) || (strict && v == least)) return;
-    const int i = atomicAdd(count, 1);
-    if (i < kCandidates) z.list[i] = candidate(v, at);
+// f(rank, candidate) for the k largest of `lists` ordered lists, kMaxList places apart, 0 behind their ends: in each, those in front of a candidate
+// are found by halving, in all lists at once.
+template <class F>
+__device__ __forceinline__ void each_best_of(const unsigned long long* list, int lists, int k, F f) {
+    const int first = 1 << (31 - __clz(k));
+#pragma unroll 1
+    for (int i = threadIdx.x; i < lists * k; i += kRowThreads) {
+        const int own = i / k, at = i - own * k;
+        const unsigned long long v = list[own * kMaxList + at];
+        int rank[kMaxCluster] = {};
+#pragma unroll 1
+        for (int half = first; half > 0; half >>= 1) {
+            unsigned long long w[kMaxCluster];
+#pragma unroll
+            for (int o = 0; o < kMaxCluster; ++o) w[o] = o < lists && rank[o] + half <= k ? list[o * kMaxList + rank[o] + half - 1] : 0ull;
+#pragma unroll
+            for (int o = 0; o < kMaxCluster; ++o) rank[o] += w[o] > v ? half : 0;
+        }
+        int all = 0;
+#pragma unroll
+        for (int o = 0; o < kMaxCluster; ++o) all += rank[o];     // in its own list too: `at` are in front of it
+        if (v != 0 && all < k) f(all, v);
+    }
 }
+// To list: the values of a quad at `at` that reach `least`, or are above it (strict).
+__device__ __forceinline__ void take(Selection& z, int* count, float4 v, int at, float least, bool strict) {
+    const float w[4] = {v.x, v.y, v.z, v.w};
+    unsigned which = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) which |= (strict ? w[i] > least : w[i] >= least) ? 1u << i : 0u;
+    if (which == 0) return;
+    int to = atomicAdd(count, __popc(which));
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (which >> i & 1u) { if (to < kCandidates) z.list[to] = candidate(w[i], at + i); ++to; }
+}
+__device__ __forceinline__ float4 alone(float v) { return make_float4(v, NAN, NAN, NAN); }       // as a quad of which nothing else is taken
 // ... of a whole part, from memory.  All threads.
 __device__ __noinline__ void take_part(Selection& z, int* count, const float* p, int n, int c0, float least, bool strict) {
     const Part part(p, n);
@@ -260,14 +377,13 @@ __device__ __noinline__ void take_part(Selection& z, int* count, const float* p,
 #pragma unroll
         for (int u = 0; u < kQuads; ++u) v[u] = load_behind(part.quads() + min(t + u * kRowThreads, part.n4 - 1));
 #pragma unroll
-        for (int u = 0; u < kQuads; ++u) {
-            if (t + u * kRowThreads >= part.n4 || !(top_of(v[u]) >= least)) continue;
-            const int at = c0 + part.head + 4 * (t + u * kRowThreads);
-            take(z, count, v[u].x, at, least, strict); take(z, count, v[u].y, at + 1, least, strict);
-            take(z, count, v[u].z, at + 2, least, strict); take(z, count, v[u].w, at + 3, least, strict);
-        }
+        for (int u = 0; u < kQuads; ++u)
+            if (t + u * kRowThreads < part.n4) take(z, count, v[u], c0 + part.head + 4 * (t + u * kRowThreads), least, strict);
     }
-    if ((int)threadIdx.x < part.n - 4 * part.n4) { const int at = part.loose(threadIdx.x); take(z, count, load_behind(part.p + at), c0 + at, least, strict); }
+    if ((int)threadIdx.x < part.n - 4 * part.n4) {
+        const int at = part.loose(threadIdx.x);
+        take(z, count, alone(load_behind(part.p + at)), c0 + at, least, strict);
+    }
 }
 // The first of those equal to `least` to list[n .. k_part).
 __device__ __noinline__ void fill_equal(Selection& z, const float* p, int part_n, int c0, float least, int n, int k_part) {
@@ -549,7 +665,7 @@ __global__ void __launch_bounds__(kRowThreads, 4) vocab_rows_kernel(VocabRows p)
     const size_t first = blockIdx.x / ranks, step = gridDim.x / ranks, mine = (p.rows - first + step - 1) / step;
     const int k = p.n_top, k_part = min(k, cn);
     if (ranks > 1) { cluster_arrive(); cluster_wait(); }          // every CTA of the cluster runs
-    if (TOP && threadIdx.x == 0) z.n_hits[0] = z.n_hits[1] = 0;
+    if (TOP && threadIdx.x == 0) z.n_hits[0] = z.n_hits[1] = z.n_list[0] = z.n_list[1] = 0;
     if (DISTILL && threadIdx.x == 0)                              // the one that joins statistics of WARPS takes a power of two of them
         for (int w = WARPS; w < kRowWarps; ++w) { sh.wm[0][w] = sh.wm[1][w] = -FLT_MAX; sh.ws[0][w] = sh.ws[1][w] = 0.0f; }
     grid_wait();
@@ -564,23 +680,23 @@ __global__ void __launch_bounds__(kRowThreads, 4) vocab_rows_kernel(VocabRows p)
     // GRAD, of the row before too, whose listed tokens are written when all of its gradient is
     float gm = 0.0f, gf = 0.0f;
     bool none = true;
-    auto value = [&](float v) { return none ? 0.0f : exp2_fast(clamp_low((v - gm) * p.c)) * gf; };
     auto write_behind = [&](size_t item) {
-        if (!none) list_write(list_warp.of(item), p.n_teacher, p.grad_logits + row_of(item) * p.stride + c0, c0, cn, up, value);
+        if (!none)
+            list_write(list_warp.of(item), p.n_teacher, p.grad_logits + row_of(item) * p.stride + c0, c0, cn, up, ProbGrad{gm, p.c, gf});
     };
     for (size_t item = 0; item < mine; ++item) {
         const size_t row = row_of(item);
         const int turn = (int)(item & 1);
         const float* x = p.logits + row * p.stride;
         const Part part(x + c0, cn);
-        Stats<ENTROPY> st;
-        float over = INFINITY, x_token = 0.0f, loose = -INFINITY;
+        Running<ENTROPY> run;
+        float over = INFINITY, least = -INFINITY, x_token = 0.0f, loose = -INFINITY;
         int token = -1;
         const bool has_loose = (int)threadIdx.x < part.n - 4 * part.n4;
         float4 again[kQuads];                                     // GRAD: the first step a second time
         if (!of_lists) {
             if (has_loose) loose = load_behind(part.p + part.loose(threadIdx.x));
-            if (!DISTILL && p.tokens != nullptr && threadIdx.x == 0 && rank == 0) {
+            if (!DISTILL && p.tokens != nullptr && threadIdx.x == kResultThread && rank == 0) {
                 token = load_behind(p.tokens + row);
                 if (token < 0 || token >= p.cols) token = -1;
                 else x_token = load_behind(x + token);
@@ -592,60 +708,56 @@ __global__ void __launch_bounds__(kRowThreads, 4) vocab_rows_kernel(VocabRows p)
                 float top = top_of(v[0]);
 #pragma unroll
                 for (int u = 1; u < kQuads; ++u) top = fmaxf(top, top_of(v[u]));
-                if (top > st.m) st.raise(top, p.c);
+                run.quads(v, top, p.c);
                 stream.next();
-#pragma unroll
-                for (int u = 0; u < kQuads; ++u) { st.term(v[u].x, p.c); st.term(v[u].y, p.c); st.term(v[u].z, p.c); st.term(v[u].w, p.c); }
                 if (TOP) {
-                    if (t == 0 && THREADS < q)                    // this thread's largest is no less than st.m, or -infinity
-                        over = unordered(max(bound_of(ordered(st.m == -FLT_MAX ? -INFINITY : st.m), k, z.bound[0]), ordered(-INFINITY)));
-                    if (top > over) {
-                        unsigned which = 0;
+                    if (q == THREADS) {                           // the sample is all
+                        run.one(loose, p.c);
+                        least = unordered(max(bound_of(ordered(run.largest()), k, z.bound[0]), ordered(-INFINITY)));
 #pragma unroll
-                        for (int u = 0; u < kQuads; ++u) which |= top_of(v[u]) > over ? 1u << u : 0u;
-                        int at = atomicAdd(&z.n_hits[turn], __popc(which));
+                        for (int u = 0; u < kQuads; ++u) {
+                            const int i = u * q + (int)threadIdx.x;
+                            if (i < part.n4) take(z, &z.n_list[turn], v[u], c0 + part.head + 4 * i, least, false);
+                        }
+                    } else {
+                        if (t <= THREADS)                         // and again a step later: fewer hits by a third
+                            over = unordered(max(bound_of(ordered(run.largest()), k, z.bound[t / THREADS]), ordered(-INFINITY)));
+                        if (top > over) {
+                            unsigned which = 0;
 #pragma unroll
-                        for (int u = 0; u < kQuads; ++u)
-                            if (which >> u & 1u) { if (at < kHits) z.hits[at] = u * q + t + (int)threadIdx.x; ++at; }
+                            for (int u = 0; u < kQuads; ++u) which |= top_of(v[u]) > over ? 1u << u : 0u;
+                            int at = atomicAdd(&z.n_hits[turn], __popc(which));
+#pragma unroll
+                            for (int u = 0; u < kQuads; ++u)
+                                if (which >> u & 1u) {
+                                    if (at < kHits) { z.hit[at] = v[u]; z.hit_at[at] = u * q + t + (int)threadIdx.x; }
+                                    ++at;
+                                }
+                        }
                     }
                 }
             }
-            st.add(loose, p.c);
+            if (!TOP || q != THREADS) run.one(loose, p.c);
             if (GRAD) load_step(part, q, 0, again);
         }
-        float least = -INFINITY;
-        if (TOP) {
-            if (threadIdx.x == 0) z.n_list[turn] = 0;
-            least = unordered(max(bound_of(ordered(st.m == -FLT_MAX ? -INFINITY : st.m), k, z.bound[1]), ordered(-INFINITY)));
-        }
+        Stats<ENTROPY> st = run.sums();
         if (!of_lists) {
             st.template join<32>(p.c);
             if (lane == 0) { sh.wm[turn][warp] = st.m; sh.ws[turn][warp] = st.s; if (ENTROPY) sh.wa[turn][warp] = st.a; }
         }
         if (TOP) {
-            const int hits = z.n_hits[turn];
             int* count = &z.n_list[turn];
-            const bool strict = !(least > over);                  // among the quads that were not noted some may equal it
-            if (hits > kHits || q <= THREADS) take_part(z, count, part.p, part.n, c0, least, false);
-            else {
+            if (q != THREADS) {
+                least = unordered(max(bound_of(ordered(run.largest()), k, z.bound[0]), ordered(-INFINITY)));
+                const int hits = z.n_hits[turn];
+                const bool strict = q > 0 && !(least > over);     // among the quads that were not noted some may equal it
+                if (hits > kHits) take_part(z, count, part.p, part.n, c0, least, false);
+                else {
 #pragma unroll 1
-                for (int i = threadIdx.x; i < hits; i += kQuads * kRowThreads) {
-                    int quad[kQuads];
-                    float4 v[kQuads];
-#pragma unroll
-                    for (int u = 0; u < kQuads; ++u) quad[u] = z.hits[min(i + u * kRowThreads, hits - 1)];
-#pragma unroll
-                    for (int u = 0; u < kQuads; ++u) v[u] = load_behind(part.quads() + quad[u]);
-#pragma unroll
-                    for (int u = 0; u < kQuads; ++u) {
-                        if (i + u * kRowThreads >= hits || !(top_of(v[u]) >= least)) continue;
-                        const int at = c0 + part.head + 4 * quad[u];
-                        take(z, count, v[u].x, at, least, strict); take(z, count, v[u].y, at + 1, least, strict);
-                        take(z, count, v[u].z, at + 2, least, strict); take(z, count, v[u].w, at + 3, least, strict);
-                    }
+                    for (int i = threadIdx.x; i < hits; i += kRowThreads) take(z, count, z.hit[i], c0 + part.head + 4 * z.hit_at[i], least, strict);
+                    if (has_loose) take(z, count, alone(loose), c0 + part.loose(threadIdx.x), least, strict);
                 }
-                if (has_loose) take(z, count, loose, c0 + part.loose(threadIdx.x), least, strict);
-            }
+            } else if (has_loose) take(z, count, alone(loose), c0 + part.loose(threadIdx.x), least, false);
         }
         if (of_lists) list_warp.arrived();                        // before anything of this row may become its gradient (grad_logits == logits)
         __syncthreads();                                          // GRAD: and all of the gradient of the row before is there
@@ -656,8 +768,8 @@ __global__ void __launch_bounds__(kRowThreads, 4) vocab_rows_kernel(VocabRows p)
         st.template join<kRowWarps>(p.c);
         int n = 0;
         if (TOP) {
-            if (threadIdx.x == 0) z.n_hits[turn] = 0;             // for the row after the next
             n = z.n_list[turn];
+            if (threadIdx.x == 0) z.n_hits[turn ^ 1] = z.n_list[turn ^ 1] = 0;       // for the next row
             if (!(st.s == st.s)) n = 0;                           // not a number: its places are not looked at
             else if (n > kCandidates || n < k_part) n = take_few(z, &z.n_list[turn], part.p, part.n, c0, least, k, k_part);
         }
@@ -667,7 +779,7 @@ __global__ void __launch_bounds__(kRowThreads, 4) vocab_rows_kernel(VocabRows p)
                 each_best(z.list, n, k_part, [&](int r, unsigned long long c) { z.best[r] = c; });
                 __syncthreads();
                 if ((int)threadIdx.x < k)
-                    asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(cluster_address(&gathered[rank * k + threadIdx.x], 0)),
+                    asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(cluster_address(&gathered[rank * kMaxList + threadIdx.x], 0)),
                                  "l"((int)threadIdx.x < min(n, k_part) ? z.best[threadIdx.x] : 0ull) : "memory");       // 0: below every candidate
             }
             if ((int)threadIdx.x < (GRAD ? ranks : 1)) {          // GRAD: all of them
@@ -691,7 +803,7 @@ __global__ void __launch_bounds__(kRowThreads, 4) vocab_rows_kernel(VocabRows p)
         }
         const float m = st.m, s = st.s, log_s = logf(s);
         auto log_prob = [&](float value) { return s == 0.0f ? -INFINITY : (value - m) * p.inv_t - log_s; };      // s == 0: nothing is left of the row
-        if (!DISTILL && threadIdx.x == 0) {
+        if (!DISTILL && threadIdx.x == kResultThread) {
             if (p.row_stats != nullptr) { p.row_stats[2 * row] = m; p.row_stats[2 * row + 1] = s; }
             if (p.logprobs != nullptr) p.logprobs[row] = token < 0 ? 0.0f : log_prob(x_token);
             if (ENTROPY) p.entropy[row] = s == 0.0f ? 0.0f : log_s - st.a / s * kLn2;
@@ -710,7 +822,7 @@ __global__ void __launch_bounds__(kRowThreads, 4) vocab_rows_kernel(VocabRows p)
                 if (p.top_logprobs != nullptr) p.top_logprobs[at + r] = log_prob(unordered((uint32_t)(c >> 32)));
             };
             if (ranks == 1) each_best(z.list, n, k, put);
-            else each_best(gathered, ranks * k, k, put);
+            else each_best_of(gathered, ranks, k, put);
         }
         if (GRAD) {
             const float sg = gradient_sum(s, list_warp.of(item).sum);
@@ -723,7 +835,7 @@ __global__ void __launch_bounds__(kRowThreads, 4) vocab_rows_kernel(VocabRows p)
             const float loss = list_loss(list, p.n_teacher, log_prob);
             if (rank == 0) list_result(p, list, row, m, s, loss);
             list_warp.ahead(item);
-        } else if (GRAD) write_part<THREADS>(part, q, p.grad_logits + row * p.stride + c0, again, loose, value);
+        } else if (GRAD) write_part<THREADS>(part, q, p.grad_logits + row * p.stride + c0, again, loose, none, ProbGrad{m, p.c, gf});
     }
     if (GRAD) {
         __syncthreads();
@@ -807,9 +919,7 @@ __global__ void __launch_bounds__(kRingThreads + 64, 1) distill_ring_kernel(Voca
         bool ok = true;
         auto write_behind = [&](size_t item) {
             const float m = stat_m[item & 3], f = stat_f[item & 3];
-            if (f != 0.0f)
-                list_write(list_warp.of(item), p.n_teacher, p.grad_logits + row_of(item) * p.stride, 0, p.cols, up,
-                           [&](float v) { return exp2_fast(clamp_low((v - m) * p.c)) * f; });
+            if (f != 0.0f) list_write(list_warp.of(item), p.n_teacher, p.grad_logits + row_of(item) * p.stride, 0, p.cols, up, ProbGrad{m, p.c, f});
         };
         for (size_t item = 0; item < mine; ++item) {
             const Part part = part_of(item);
@@ -847,7 +957,7 @@ __global__ void __launch_bounds__(kRingThreads + 64, 1) distill_ring_kernel(Voca
         const Part part = part_of(item);
         const bool has_loose = (int)threadIdx.x < part.n - 4 * part.n4;
         const float loose = has_loose ? load_behind(part.p + part.loose(threadIdx.x)) : -INFINITY;
-        Stats<false> st;
+        Running<false> run;
         int at_slot = slot;
         uint32_t at_parity = parity;
         if (!of_lists) {
@@ -856,17 +966,19 @@ __global__ void __launch_bounds__(kRingThreads + 64, 1) distill_ring_kernel(Voca
                 if (ok && !mbar_wait_warp(smem_u32(&full[at_slot]), at_parity, &gave_up)) { ok = false; gone(); }
                 float4 v[2];
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const int i = u * kRingThreads + (int)threadIdx.x;
-                    v[u] = c * kChunkQuads + i < part.n4 ? ring[at_slot * kChunkQuads + i] : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-                }
-                const float top = fmaxf(top_of(v[0]), top_of(v[1]));
-                if (top > st.m) st.raise(top, p.c);
+                for (int u = 0; u < 2; ++u) v[u] = ring[at_slot * kChunkQuads + u * kRingThreads + threadIdx.x];
+                if ((c + 1) * kChunkQuads > part.n4) {
 #pragma unroll
-                for (int u = 0; u < 2; ++u) { st.term(v[u].x, p.c); st.term(v[u].y, p.c); st.term(v[u].z, p.c); st.term(v[u].w, p.c); }
+                    for (int u = 0; u < 2; ++u)
+                        if (c * kChunkQuads + u * kRingThreads + (int)threadIdx.x >= part.n4) v[u] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+                }
+                run.quads(v, fmaxf(top_of(v[0]), top_of(v[1])), p.c);
                 if (++at_slot == kRingChunks) { at_slot = 0; at_parity ^= 1u; }
             }
-            st.add(loose, p.c);
+            run.one(loose, p.c);
+        }
+        Stats<false> st = run.sums();
+        if (!of_lists) {
             st.join<32>(p.c);
             if (lane == 0) { wm[turn][warp] = st.m; ws[turn][warp] = st.s; }
         }
@@ -886,8 +998,8 @@ __global__ void __launch_bounds__(kRingThreads + 64, 1) distill_ring_kernel(Voca
             continue;
         }
         if (threadIdx.x == 0) { stat_m[item & 3] = m; stat_f[item & 3] = f; }
-        auto value = [&](float v) { return f == 0.0f ? 0.0f : exp2_fast(clamp_low((v - m) * p.c)) * f; };
-        if (has_loose) p.grad_logits[row * p.stride + part.loose(threadIdx.x)] = value(loose);
+        const ProbGrad value = {m, p.c, f};
+        if (has_loose) p.grad_logits[row * p.stride + part.loose(threadIdx.x)] = f == 0.0f ? 0.0f : value(loose);
 #pragma unroll 1
         for (int c = 0; c < chunks; ++c) {
 #pragma unroll
@@ -895,8 +1007,7 @@ __global__ void __launch_bounds__(kRingThreads + 64, 1) distill_ring_kernel(Voca
                 const int i = u * kRingThreads + (int)threadIdx.x;
                 if (c * kChunkQuads + i >= part.n4) continue;
                 float4& at = ring[slot * kChunkQuads + i];
-                const float4 v = at;
-                at = make_float4(value(v.x), value(v.y), value(v.z), value(v.w));
+                at = f == 0.0f ? make_float4(0.f, 0.f, 0.f, 0.f) : quad_of(at, value);
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
@@ -967,13 +1078,11 @@ __global__ void __launch_bounds__(kRowThreads, 4) vocab_grad_kernel(VocabGrad p)
             k1 = -h * kLn2 / s;
             __syncthreads();        // the token's logit is read before any of the row is written (grad_logits may be logits); other tiles' are not used
         }
-        auto value = [&](float at) {
-            const float d = clamp_low((at - m) * p.c);
-            return none ? 0.0f : exp2_fast(d) * (DISTILL ? k0 : fmaf(k1, d, k0));
-        };
-        write_part<kRowThreads>(part, q, g, v, loose, value);
+        const EntropyGrad with_entropy = {m, p.c, k0, k1};
+        if (DISTILL) write_part<kRowThreads>(part, q, g, v, loose, none, ProbGrad{m, p.c, k0});
+        else write_part<kRowThreads>(part, q, g, v, loose, none, with_entropy);
         __syncthreads();
-        if (!DISTILL && threadIdx.x == 0 && !none && token >= c0 && token < c0 + cn) g[token - c0] = value(x_token) + up;
+        if (!DISTILL && threadIdx.x == 0 && !none && token >= c0 && token < c0 + cn) g[token - c0] = with_entropy(x_token) + up;
         if (DISTILL && warp == 0 && !none) {
             copies_wait<0>();
             __syncwarp();
