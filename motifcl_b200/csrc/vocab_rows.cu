@@ -157,9 +157,6 @@ struct Part {
 // The quads of a thread: those at threadIdx.x modulo the threads, kQuads of them a step, a quarter of the part apart, so that the first step is a
 // sample of the part.  The distance depends on the part's length alone: a thread meets the same places whatever a row's alignment is.
 __device__ __forceinline__ int quarter_of(int n, int threads) { return (((n >> 2) + kQuads - 1) / kQuads + threads - 1) / threads * threads; }
-__device__ __forceinline__ void copy_async16(void* to, const void* from) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
-}
 __device__ __forceinline__ void copy_async4(void* to, const void* from) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
 }
@@ -172,48 +169,70 @@ __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_grou
 constexpr int kAhead = 2;
 template <int THREADS, class P>
 struct Stream {
-    float4* ring;                      // [kAhead][kQuads][THREADS]
+    // The addresses are kept, not formed anew for every copy: that took 80 instructions of a step's 190.
+    static constexpr uint32_t kPlace = THREADS * 16, kSlot = kQuads * kPlace;
     const P& part;
-    Part at;                           // being fetched
     size_t next_item, items;
-    int q, t, slot;
+    const char* from;                  // this thread's first quad of the next step to fetch
+    size_t stretch;                    // bytes of a quarter
+    uint32_t mine, in, out;            // shared memory: this thread's place in the first slot; offsets of the slots to fill and to take
+    int q, t, whole, n4;               // being fetched: its step, from which on a step is not whole, its quads
     __device__ __forceinline__ Stream(void* shared, const P& parts, size_t count, int longest)
-        : ring(static_cast<float4*>(shared)), part(parts), at(parts(0)), next_item(0), items(count), q(quarter_of(longest, THREADS)), t(0), slot(0) {
-        for (int i = 0; i < kAhead; ++i) fetch(i);
+        : part(parts), next_item(0), items(count), mine((uint32_t)__cvta_generic_to_shared(shared) + threadIdx.x * 16), in(0), out(0), q(quarter_of(longest, THREADS)) {
+        stretch = (size_t)q * 16;
+        if (q == 0) items = 0;
+        start();
+        for (int i = 0; i < kAhead; ++i) fetch();
     }
-    __device__ __forceinline__ void fetch(int to) {
-        if (next_item < items && q > 0) {
-            const int i = t + (int)threadIdx.x;
-            const float4* from = at.quads() + i;
-            float4* place = ring + to * kQuads * THREADS + threadIdx.x;
-            const bool whole = t + (kQuads - 1) * q + THREADS <= at.n4;
-#pragma unroll
-            for (int u = 0; u < kQuads; ++u)
-                if (whole || u * q + i < at.n4) copy_async16(place + u * THREADS, from + u * q);
-            t += THREADS;
-            if (t >= q) {
-                t = 0;
-                if (++next_item < items) at = part(next_item);
+    __device__ __forceinline__ void start() {
+        if (next_item >= items) return;
+        const Part at = part(next_item);
+        from = reinterpret_cast<const char*>(at.quads() + threadIdx.x);
+        n4 = at.n4;
+        t = 0;
+        whole = at.n4 - (kQuads - 1) * q - THREADS;
+    }
+    template <int U>
+    __device__ __forceinline__ void copy(uint32_t to, const char* at) {
+        asm volatile("cp.async.cg.shared.global [%0+%2], [%1], 16;" ::"r"(to), "l"(at), "n"(U * (int)kPlace) : "memory");
+    }
+    template <int U>
+    __device__ __forceinline__ void load(float4& v) {
+        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4+%5];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(mine + out), "n"(U * (int)kPlace) : "memory");
+    }
+    __device__ __forceinline__ void fetch() {
+        if (next_item < items) {
+            const uint32_t to = mine + in;
+            const char *b = from + stretch, *c = b + stretch, *d = c + stretch;
+            if (t <= whole) {
+                copy<0>(to, from); copy<1>(to, b); copy<2>(to, c); copy<3>(to, d);
+            } else {
+                const int i = t + (int)threadIdx.x;
+                if (i < n4) copy<0>(to, from);
+                if (i + q < n4) copy<1>(to, b);
+                if (i + 2 * q < n4) copy<2>(to, c);
+                if (i + 3 * q < n4) copy<3>(to, d);
             }
+            from += THREADS * 16;
+            t += THREADS;
+            if (t >= q) { ++next_item; start(); }
         }
         copies_end();
+        in = in + kSlot < kAhead * kSlot ? in + kSlot : 0;
     }
     // step `now` of a part with n4 quads: -infinity behind the end.  next() follows when the values have been used
-    __device__ __forceinline__ void take(int now, int n4, float4 (&v)[kQuads]) {
+    __device__ __forceinline__ void take(int now, int quads, float4 (&v)[kQuads]) {
         copies_wait<kAhead - 1>();
-        const float4* place = ring + slot * kQuads * THREADS + threadIdx.x;
-#pragma unroll
-        for (int u = 0; u < kQuads; ++u) v[u] = place[u * THREADS];
-        if (now + (kQuads - 1) * q + THREADS <= n4) return;
+        load<0>(v[0]); load<1>(v[1]); load<2>(v[2]); load<3>(v[3]);
+        out = out + kSlot < kAhead * kSlot ? out + kSlot : 0;
+        if (now + (kQuads - 1) * q + THREADS <= quads) return;
 #pragma unroll
         for (int u = 0; u < kQuads; ++u)
-            if (u * q + now + (int)threadIdx.x >= n4) v[u] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+            if (u * q + now + (int)threadIdx.x >= quads) v[u] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
     }
-    __device__ __forceinline__ void next() {
-        fetch(slot);
-        slot = slot + 1 < kAhead ? slot + 1 : 0;
-    }
+    __device__ __forceinline__ void next() { fetch(); }
 };
+static_assert(kQuads == 4, "a step's copies are written out");
 constexpr size_t kStreamBytes = (size_t)kAhead * kQuads * kRowThreads * sizeof(float4);
 
 // g[i] = f(x[i]) over a part; v is the first step, loaded by the caller ahead of what f waits for.  By loads and stores of the threads themselves:
