@@ -1295,11 +1295,16 @@ int mcl_cuda_rmsnorm_backward_weight(mcl_cuda_ctx* ctx, const float* x, const fl
     if (cols > 1024) ctx->launches += 1;     // a row pass and a column pass
     return MCL_CUDA_OK;
 }
+static int check_norm(mcl_cuda_ctx* ctx, const char* op, size_t rows, size_t cols) {
+    MCL_TRY(check_rows(ctx, op, rows, cols));
+    if (cols > 0x40000000ull) return fail(ctx, MCL_CUDA_EINVAL, std::string(op) + " dimension is too large");       // a thread's next column is an int
+    return MCL_CUDA_OK;
+}
 int mcl_cuda_layernorm(mcl_cuda_ctx* ctx, const float* x, const float* weight, const float* bias, float* out, float* row_stats, size_t rows,
                        size_t cols, float eps) {
     MCL_NEED_CTX(ctx);
     const char* op = "layernorm";
-    MCL_TRY(check_rows(ctx, op, rows, cols));
+    MCL_TRY(check_norm(ctx, op, rows, cols));
     if (!std::isfinite(eps) || eps < 0.0f) return fail(ctx, MCL_CUDA_EINVAL, "layernorm requires non-negative finite eps");
     MCL_TRY(check_ptr(ctx, op, "x", x, 4));
     MCL_TRY(check_ptr(ctx, op, "weight", weight, 4));
@@ -1314,7 +1319,7 @@ int mcl_cuda_layernorm_backward(mcl_cuda_ctx* ctx, const float* x, const float* 
                                 float* grad_x, float* grad_weight, float* grad_bias, size_t rows, size_t cols) {
     MCL_NEED_CTX(ctx);
     const char* op = "layernorm backward";
-    MCL_TRY(check_rows(ctx, op, rows, cols));
+    MCL_TRY(check_norm(ctx, op, rows, cols));
     MCL_TRY(check_ptr(ctx, op, "x", x, 4));
     MCL_TRY(check_ptr(ctx, op, "weight", weight, 4));
     MCL_TRY(check_ptr(ctx, op, "grad_out", grad_out, 4));
@@ -1419,6 +1424,7 @@ int mcl_cuda_softmax_cross_entropy_backward(mcl_cuda_ctx* ctx, const float* logi
 namespace {
 int check_vocab(mcl_cuda_ctx* ctx, const char* op, const float* logits, size_t rows, size_t cols, size_t row_stride, float temperature) {
     MCL_TRY(check_rows(ctx, op, rows, cols));
+    if (cols > 0x40000000ull) return fail(ctx, MCL_CUDA_EINVAL, std::string(op) + " dimension is too large");       // places of four quads on are ints
     if (row_stride < cols) return fail(ctx, MCL_CUDA_EINVAL, std::string(op) + " requires row_stride >= cols");
     if (row_stride > (size_t)-1 / sizeof(float) / rows) return fail(ctx, MCL_CUDA_EINVAL, std::string(op) + " dimension is too large");
     if (!(temperature > 0.0f) || !std::isfinite(temperature) || !(1.0f / temperature >= 1e-30f) || !(1.0f / temperature <= 1e30f))

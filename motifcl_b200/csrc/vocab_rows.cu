@@ -484,7 +484,6 @@ struct VocabRows {
 struct __align__(16) TeacherList {
     int id[kMaxList];                  // outside [0, cols): no entry
     float t[kMaxList], log_t[kMaxList], x[kMaxList];                // probabilities, their logarithms, the student's logits
-    float g[kMaxList];                 // the listed tokens' gradients (list_take_off)
     float sum;                         // of the exponentials; 0: an empty list
     bool twice;                        // a token is named more than once
 };
@@ -524,42 +523,6 @@ __device__ __forceinline__ void list_terms(TeacherList& l, const P& p) {
     if (lane == 0) l.sum = sum;
     __syncwarp();
 }
-// Takes the listed tokens' probabilities, times `up`, off their gradients: where(i) is the gradient of entry i, or null.  Entries that name the same
-// token find out through it: each leaves its number there, and one of them finds its own; that one takes off all of theirs, in their order.
-template <class W>
-__device__ __forceinline__ void list_take_off(TeacherList& l, int n, float up, W where) {
-    const int lane = threadIdx.x & 31;
-    for (int i = lane; i < n; i += 32) {
-        volatile float* g = where(i);
-        if (g != nullptr) l.g[i] = *g;
-    }
-    __syncwarp();
-    for (int i = lane; i < n; i += 32) {
-        volatile int* g = reinterpret_cast<volatile int*>(where(i));
-        if (g != nullptr) *g = i;
-    }
-    __syncwarp();
-    unsigned last = 0;                 // bit j: entry lane + 32 j found its number
-    bool twice = false;
-    for (int i = lane, j = 0; i < n; i += 32, ++j) {
-        volatile int* g = reinterpret_cast<volatile int*>(where(i));
-        if (g == nullptr) continue;
-        if (*g == i) last |= 1u << j;
-        else twice = true;
-    }
-    twice = __any_sync(0xffffffffu, twice);
-    for (int i = lane, j = 0; i < n; i += 32, ++j) {
-        if (!(last >> j & 1u)) continue;
-        float t = l.t[i];
-        if (twice) {
-            t = 0.0f;
-            for (int o = 0; o < n; ++o)
-                if (l.id[o] == l.id[i]) t += l.t[o];
-        }
-        *where(i) = l.g[i] - t * up;
-    }
-    __syncwarp();
-}
 template <class F>
 __device__ __forceinline__ float list_loss(const TeacherList& l, int n, F log_prob) {
     float loss = 0.0f;
@@ -589,10 +552,10 @@ __device__ __forceinline__ bool list_twice(const TeacherList& l, const P& p) {
     }
     return __any_sync(0xffffffffu, twice);
 }
-// g[id] of the listed tokens in [c0, c0 + cn), behind the rest of g, from the student's logits: the first entry that names a token takes all of
-// its entries' probabilities off, in their order.
+// The gradients of the listed tokens in [c0, c0 + cn), behind the rest of g: f(entry, place) for the first entry that names a token, and the
+// probabilities of all its entries, in their order, to be taken off.
 template <class F>
-__device__ __forceinline__ void list_write(const TeacherList& l, int n, float* g, int c0, int cn, float up, F value) {
+__device__ __forceinline__ void each_listed(const TeacherList& l, int n, int c0, int cn, F f) {
     for (int i = threadIdx.x & 31; i < n; i += 32) {
         const int id = l.id[i];
         if (id < c0 || id - c0 >= cn) continue;
@@ -604,8 +567,13 @@ __device__ __forceinline__ void list_write(const TeacherList& l, int n, float* g
                 if (l.id[j] == id) { t += l.t[j]; first = first && j >= i; }
             if (!first) continue;
         }
-        g[id - c0] = value(l.x[i]) - t * up;
+        f(i, id - c0, t);
     }
+}
+// From the student's logits:
+template <class F>
+__device__ __forceinline__ void list_write(const TeacherList& l, int n, float* g, int c0, int cn, float up, F value) {
+    each_listed(l, n, c0, cn, [&](int i, int at, float t) { g[at] = value(l.x[i]) - t * up; });
 }
 // The lists of items 0, 1, ... of a CTA: row(i) is an item's row.
 template <int LISTS, class P, class R>
@@ -1108,7 +1076,10 @@ __global__ void __launch_bounds__(kRowThreads, 4) vocab_grad_kernel(VocabGrad p)
             for (int i = lane; i < p.n_teacher; i += 32)
                 if (list.id[i] < 0 || list.id[i] >= p.cols) list.t[i] = -INFINITY;
             list_terms(list, p);
-            list_take_off(list, p.n_teacher, up, [&](int i) -> float* { return list.id[i] >= c0 && list.id[i] - c0 < cn ? g + (list.id[i] - c0) : nullptr; });
+            const bool twice = list_twice(list, p);
+            if (lane == 0) list.twice = twice;
+            __syncwarp();
+            each_listed(list, p.n_teacher, c0, cn, [&](int, int at, float t) { g[at] -= t * up; });      // p is there
         }
     }
 }
