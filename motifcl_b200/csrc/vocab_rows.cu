@@ -1,6 +1,11 @@
 // What rows of logits say about tokens: log probabilities of given tokens with the entropy of the row and its most probable
 // tokens, the gradient of both, and the loss of a student against the tokens that a teacher kept, with its gradient.
 //
+// Bound by memory: a forward call reads the logits once, a gradient reads them and writes as much; next to that the issue slots, of which an fp32 value takes
+// 11.8 thread-instructions where only its statistics are wanted (pairs of values an instruction) and 20.5 with the 20 largest sought.
+// 4096 x 32000 (524 MB; a copy would take 81.5 us for its bytes, 163 us for read and written): log probabilities and entropy 78 us, with the 20 most probable
+// tokens 110 us, their gradient 161 us; distillation from lists of 64: loss 80 us, loss and gradient in one call 191 us, gradient from kept statistics 176 us.
+//
 // With T the temperature, m the largest logit of a row and d_c = (x_c - m) / T:
 //     s = sum exp(d_c)      log p_c = d_c - ln s      H = ln s - (sum exp(d_c) d_c) / s
 // so that both parts of H have one sign and nothing cancels.  m and s are kept apart (row_stats): their sum m / T + ln s would lose
@@ -11,6 +16,7 @@
 #include "tc_ptx.cuh"
 
 #include <cfloat>
+#include <climits>
 #include <cmath>
 
 namespace mcl {
@@ -19,10 +25,10 @@ namespace {
 constexpr int kRowThreads = 256;
 constexpr int kRowWarps = kRowThreads / 32;
 constexpr int kResultThread = kRowThreads - 32;        // writes a row's results: the first of the warp that has least to do at the end
-constexpr int kQuads = 4;              // of a thread in flight
+constexpr int kQuads = 4;              // of a thread in a step
 constexpr int kMaxList = kVocabListMax;
 constexpr int kMaxCluster = 8;
-constexpr int kHits = 768;             // quads with a value above a row's first bounds
+constexpr int kHits = 928;             // quads with a value above a row's first bounds
 constexpr int kCandidates = 512;       // values that reach its last one
 constexpr float kLn2 = 0.69314718f;    // ln 2 to fp32
 
@@ -166,10 +172,12 @@ __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_grou
 
 // Parts on their way: a thread copies the quads that it will work on itself, kAhead steps ahead and over the end of a part, so
 // that nothing waits for another thread and memory is busy while a row is finished.  part(i): the i-th of `items`, of at most `longest` logits.
+// With 4 CTAs an SM has 128 KB on their way.  4096 x 32000 alone / with 20 tops: 78 / 110 us; three steps ahead 84 / 138 (three CTAs an SM); half the threads,
+// eight quads each 84 / 104 but 29 us instead of 27 for 777 x 50003; bulk copies and their barriers 81 / 117 (before the addresses were kept: 78 / 112).
 constexpr int kAhead = 2;
 template <int THREADS, class P>
 struct Stream {
-    // The addresses are kept, not formed anew for every copy: that took 80 instructions of a step's 190.
+    // The addresses are kept, not formed anew for every copy: 112 us then for 4096 x 32000 with 20 tops, 108.5 so.
     static constexpr uint32_t kPlace = THREADS * 16, kSlot = kQuads * kPlace;
     const P& part;
     size_t next_item, items;
@@ -236,7 +244,7 @@ static_assert(kQuads == 4, "a step's copies are written out");
 constexpr size_t kStreamBytes = (size_t)kAhead * kQuads * kRowThreads * sizeof(float4);
 
 // g[i] = f(x[i]) over a part; v is the first step, loaded by the caller ahead of what f waits for.  By loads and stores of the threads themselves:
-// asynchronous copies behind stores wait in the same queue (4096 x 32000: 184 us, 163 so).
+// asynchronous copies behind stores wait in the same queue (4096 x 32000: 184 us, 161 so).
 __device__ __forceinline__ void load_step(const Part& part, int q, int t, float4 (&v)[kQuads]) {
 #pragma unroll
     for (int u = 0; u < kQuads; ++u) {
@@ -467,7 +475,7 @@ struct VocabRows {
     float* entropy;
     int* top_ids;
     float* top_logprobs;
-    int n_top;
+    int n_top, last_bound;             // the last step behind which a bound is taken
     float* row_stats;
     const int* teacher_ids;
     const float* teacher_logits;
@@ -632,8 +640,10 @@ __device__ __forceinline__ void list_result(const VocabRows& p, const TeacherLis
 // One row at a time on a CTA, or a row on a cluster's CTAs where there are few.
 // TOP: a thread's first step is a sample of the row; the quads with something above the bound that it gives are noted as the row goes by, and
 // looked at again under the bound of all that the threads have seen.
-// LIST, GRAD: the last warp has the teacher's lists and forms the losses; the row goes by a second time (out of L2), becomes its gradient, and that
-// warp takes the listed tokens' probabilities off it while the next row is at work.
+// That stays behind 1 % of the values of a long row and costs no second look at memory: 30 us of 110, which are issue slots (71 % of them
+// busy) and the barriers of a row.  Where more than kHits quads are noted (lists of 128 of long rows) the row is read again.
+// LIST, GRAD: the last warp has the teacher's lists and forms the losses.  GRAD: the row goes by a second time (out of L2, where rows are few or short; long
+// ones go through the ring below), becomes its gradient, and that warp writes the listed tokens' gradients while the next row is at work.
 enum RowWork { kPlain, kTop, kList, kGrad };
 template <bool ENTROPY, RowWork WORK>
 __global__ void __launch_bounds__(kRowThreads, 4) vocab_rows_kernel(VocabRows p) {
@@ -707,8 +717,9 @@ __global__ void __launch_bounds__(kRowThreads, 4) vocab_rows_kernel(VocabRows p)
                             if (i < part.n4) take(z, &z.n_list[turn], v[u], c0 + part.head + 4 * i, least, false);
                         }
                     } else {
-                        if (t <= THREADS)                         // and again a step later: fewer hits by a third
-                            over = unordered(max(bound_of(ordered(run.largest()), k, z.bound[t / THREADS]), ordered(-INFINITY)));
+                        const int past = t / THREADS;
+                        if (past <= p.last_bound && (past & (past + 1)) == 0)
+                            over = unordered(max(bound_of(ordered(run.largest()), k, z.bound[__popc(past) & 1]), ordered(-INFINITY)));
                         if (top > over) {
                             unsigned which = 0;
 #pragma unroll
@@ -735,7 +746,8 @@ __global__ void __launch_bounds__(kRowThreads, 4) vocab_rows_kernel(VocabRows p)
         if (TOP) {
             int* count = &z.n_list[turn];
             if (q != THREADS) {
-                least = unordered(max(bound_of(ordered(run.largest()), k, z.bound[0]), ordered(-INFINITY)));
+                const int bounds = 32 - __clz(min(q / THREADS, p.last_bound + 1));       // taken on the way
+                least = unordered(max(bound_of(ordered(run.largest()), k, z.bound[bounds & 1]), ordered(-INFINITY)));
                 const int hits = z.n_hits[turn];
                 const bool strict = q > 0 && !(least > over);     // among the quads that were not noted some may equal it
                 if (hits > kHits) take_part(z, count, part.p, part.n, c0, least, false);
@@ -833,8 +845,9 @@ __global__ void __launch_bounds__(kRowThreads, 4) vocab_rows_kernel(VocabRows p)
 // ---- loss and gradient of long rows in one pass ---------------------------------------------------------------------------
 // A row comes to shared memory once, in chunks by bulk copies, becomes its gradient there, and goes out by bulk copies: a ring of chunks in which the
 // next row comes while this one is at work and the one before goes.  The threads themselves neither load nor store: behind their own stores all
-// of an SM's memory instructions, those on shared memory among them, waited two thirds of the time (the row a second time out of L2: 300 us for 4096 x
-// 32000 with four rows on an SM, which L2 does not hold, 400 with two).
+// of an SM's memory instructions, those on shared memory among them, waited two thirds of the time.  4096 x 32000 with lists of 64: 191 us, 85 % of the copy's
+// rate; the row a second time out of L2 300 us with four rows on an SM, of which L2 keeps none, 325 with three, 398 with two, 549 with one; a row in shared memory
+// with the threads' own copies and stores 219.
 // Two more warps: one has the teacher's lists and forms the losses; one issues the copies and writes the listed tokens' gradients a row behind.
 constexpr int kRingThreads = 512;      // that work on rows
 constexpr int kRingWarps = kRingThreads / 32;
@@ -931,6 +944,11 @@ __global__ void __launch_bounds__(kRingThreads + 64, 1) distill_ring_kernel(Voca
         if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
         __syncwarp();
         write_behind(mine - 1);
+        if (*(volatile int*)&gave_up) {
+            // loads that are still in flight land before the shared memory is released
+            const unsigned long long t0 = clock64();
+            while (clock64() - t0 < 2000000ull) {}
+        }
         return;
     }
     const bool of_lists = warp == kRingWarps;
@@ -1023,6 +1041,7 @@ struct VocabGrad {
 };
 
 // dx_c = e_c (k0 + k1 d_c) + (what the named tokens add), with e_c = 2^((x_c - m) c): p_c enters through 1 / s in k0 and k1.
+// Bound by memory, read and write: 4096 x 32000 in 161 us, a copy's rate; from lists of 64 176 us, as a CTA's writing ends in one warp's work.
 // DISTILL: the first warp has an item's list on its way from the start, and takes the listed tokens' probabilities off when the rest is written.
 template <bool DISTILL>
 __global__ void __launch_bounds__(kRowThreads, 4) vocab_grad_kernel(VocabGrad p) {
@@ -1080,6 +1099,7 @@ __global__ void __launch_bounds__(kRowThreads, 4) vocab_grad_kernel(VocabGrad p)
             if (lane == 0) list.twice = twice;
             __syncwarp();
             each_listed(list, p.n_teacher, c0, cn, [&](int, int at, float t) { g[at] -= t * up; });      // p is there
+            __syncwarp();                                         // before the next item's list comes
         }
     }
 }
@@ -1097,7 +1117,7 @@ cudaError_t launch_rows(void (*kern)(P), unsigned grid, int threads, int cluster
     cfg.attrs = at; cfg.numAttrs = cluster > 1 ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kern, p);
 }
-// CTAs of a row: as many as leave none of the SMs idle, with 2048 logits each at least
+// CTAs of a row: as many as leave none of the SMs idle, with 2048 logits each at least (one row of 32000: 6.8 us by eight, 16 rows 7.5)
 int row_cluster(size_t rows, int cols, int sm_count) {
     int n = 1;
     while (n < kMaxCluster && rows * 2 * n <= 2 * (size_t)sm_count && cols / (2 * n) >= 2048) n *= 2;
@@ -1105,6 +1125,10 @@ int row_cluster(size_t rows, int cols, int sm_count) {
 }
 cudaError_t launch_forward(VocabRows& p, int sm_count, cudaStream_t stream) {
     p.cluster = row_cluster(p.rows, p.cols, sm_count);
+    // Bounds after 1, 2, 4, 8, ... steps, between two of which there are as many hits again; after 1 and 2 only where a barrier and a bound are more than the
+    // hits they save.  All of them / two, k = 20: 4096 x 32000 (8 steps) 112 / 110 us, 2000 x 50003 82 / 86, 600 x 128256 69 / 122; k = 64:
+    // 147 / 139, 99 / 138, 76 / 140; k = 128, 4096 x 32000: 231 / 302, as two leave more than kHits.
+    p.last_bound = p.n_top > 64 || p.cols / p.cluster > 10 * 4 * kQuads * kRowThreads ? INT_MAX - 1 : 1;
     const size_t cap = (size_t)sm_count * 4;
     const unsigned grid = p.cluster > 1 ? (unsigned)(p.rows * p.cluster) : (unsigned)(p.rows < cap ? p.rows : cap);
     const bool distill = p.n_teacher > 0;

@@ -218,6 +218,8 @@ def test_refusals(ctx):
     refused("non-zero", ln, f(R, N), f(N), f(N), f(R, N), None, 0, N, 1e-5)
     refused("non-zero", ln, f(R, N), f(N), f(N), f(R, N), None, R, 0, 1e-5)
     refused("too large", ln, f(R, N), f(N), f(N), f(R, N), None, R, 1 << 31, 1e-5)
+    refused("too large", ln, f(R, N), f(N), f(N), f(R, N), None, R, (1 << 30) + 1, 1e-5)
+    refused("too large", bw, f(R, N), f(N), f(R, N), f(R, 2), f(R, N), None, None, R, (1 << 30) + 1)
     for eps in (-1e-6, math.nan, math.inf):
         refused("eps", ln, f(R, N), f(N), f(N), f(R, N), None, R, N, eps)
     refused("x is NULL", ln, None, f(N), f(N), f(R, N), None, R, N, 1e-5)

@@ -161,6 +161,19 @@ def test_token_logprobs_of_masked_and_extreme_rows(ctx, R, V, k, T, rounded):
     check_logprobs(ctx, x, stride, k, T, tokens)
 
 
+@pytest.mark.parametrize("R,V,k,rounded", [(160, 90001, 20, False), (155, 50000, 128, False), (160, 70003, 64, True), (150, 150000, 1, False), (300, 24001, 100, True)])
+def test_top_tokens_of_rows_of_many_steps(ctx, R, V, k, rounded):
+    """More rows than clusters take, each long enough for several bounds on the way."""
+    x, stride = make_logits(R, V, 1, 0, seed=6, rounded=rounded)
+    special_rows(x)
+    x[8] = torch.arange(V, 0, -1, device=x.device) * (20.0 / V)      # descending: the first bound is the last
+    x[9, V // 2:] += 30.0                                           # everything that counts behind the middle
+    x[10].copy_(torch.where(torch.arange(V, device=x.device) % 4096 < 1024, x[10] + 9.0, x[10]))
+    tokens = torch.full((R,), 0)
+    tokens[5], tokens[6], tokens[7] = V - 1, V // 2, 1
+    check_logprobs(ctx, x, stride, k, 1.0, tokens)
+
+
 def test_top_tokens_where_one_thread_has_all_large_values(ctx):
     """More values above a bound from the threads' largest than are collected at once."""
     V, k = 32000, 128
@@ -602,6 +615,7 @@ def test_refusals(ctx):
     refused("row_stride", lp, x, tok, f(R), None, None, None, None, R, V, row_stride=V - 1)
     refused("too large", lp, x, tok, f(R), None, None, None, None, R, V, row_stride=1 << 62)
     refused("too large", lp, x, tok, f(R), None, None, None, None, R, 1 << 31)
+    refused("too large", lp, x, tok, f(R), None, None, None, None, R, (1 << 30) + 1)
     for T in (0.0, -1.0, math.nan, math.inf, 1e-35, 1e35):
         refused("temperature", lp, x, tok, f(R), None, None, None, None, R, V, 0, T)
     refused("n_top", lp, x, tok, f(R), None, big, f(R, 200), None, R, V, 129)
