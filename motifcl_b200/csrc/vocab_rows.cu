@@ -15,6 +15,7 @@
 #include "kernels.h"
 #include "tc_ptx.cuh"
 
+#include <algorithm>
 #include <cfloat>
 #include <climits>
 #include <cmath>
@@ -492,6 +493,7 @@ struct VocabRows {
 struct __align__(16) TeacherList {
     int id[kMaxList];                  // outside [0, cols): no entry
     float t[kMaxList], log_t[kMaxList], x[kMaxList];                // probabilities, their logarithms, the student's logits
+    float g[kMaxList];                 // the gradients at the entries (ring)
     float sum;                         // of the exponentials; 0: an empty list
     bool twice;                        // a token is named more than once
 };
@@ -576,6 +578,19 @@ __device__ __forceinline__ void each_listed(const TeacherList& l, int n, int c0,
             if (!first) continue;
         }
         f(i, id - c0, t);
+    }
+}
+// The same at every entry, from the student's logits: entries that name the same token get the same.
+template <class F>
+__device__ __forceinline__ void list_gradients(TeacherList& l, int n, float up, F value) {
+    for (int i = threadIdx.x & 31; i < n; i += 32) {
+        float t = l.t[i];
+        if (l.twice) {
+            t = 0.0f;
+            for (int j = 0; j < n; ++j)
+                if (l.id[j] == l.id[i]) t += l.t[j];
+        }
+        l.g[i] = value(l.x[i]) - t * up;
     }
 }
 // From the student's logits:
@@ -851,15 +866,15 @@ __global__ void __launch_bounds__(kRowThreads, 4) vocab_rows_kernel(VocabRows p)
 // Two more warps: one has the teacher's lists and forms the losses; one issues the copies and writes the listed tokens' gradients a row behind.
 constexpr int kRingThreads = 512;      // that work on rows
 constexpr int kRingWarps = kRingThreads / 32;
-constexpr int kChunkQuads = 2 * kRingThreads;
-constexpr int kRingChunks = 13;
-// Chunks of a row.  At most: the last of a row is loaded when the one kRingChunks - 2 before it has left, which has to be of the row before.  At least: when a row's
-// statistics are there, its last chunk is, so the copying warp is at work on the row before or this one, and lists and statistics of three rows before are free.
-constexpr int kRingMost = kRingChunks - 2;
-constexpr int kRingLeast = 7;
-constexpr int kRingLists = 5;
-constexpr size_t kRingBytes = (size_t)kRingChunks * kChunkQuads * sizeof(float4);
+constexpr size_t kRingBytes = 208 * 1024;
+constexpr int kRingMost = 12;          // chunks of a row
+constexpr int kRingAhead = 2;          // rows in the ring beside the one that goes out, at most
+constexpr int kRingSlots = (kRingAhead + 1) * kRingMost;
+constexpr int kRingLists = 4 + kRingAhead;                        // from the row before the one that goes out to two behind the last one in the ring
 constexpr int kRingErr = 61;
+struct Ring {
+    int chunk, chunks, slots;          // quads of a chunk, chunks of a row, chunks of the ring
+};
 __device__ __forceinline__ void bulk_load(uint32_t to, const void* from, uint32_t bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(to), "l"(from), "r"(bytes), "r"(bar) : "memory");
 }
@@ -867,19 +882,20 @@ __device__ __forceinline__ void bulk_store(void* to, uint32_t from, uint32_t byt
     asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(to), "r"(from), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void bulk_end() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
-__global__ void __launch_bounds__(kRingThreads + 64, 1) distill_ring_kernel(VocabRows p, int chunks) {
+__global__ void __launch_bounds__(kRingThreads + 64, 1) distill_ring_kernel(VocabRows p, Ring r) {
     grid_release();
     extern __shared__ __align__(16) unsigned char dynamic[];
     float4* ring = reinterpret_cast<float4*>(dynamic);
-    __shared__ float wm[2][kRingWarps], ws[2][kRingWarps], stat_m[4], stat_f[4];
+    __shared__ float wm[2][kRingWarps], ws[2][kRingWarps];
+    __shared__ bool stat_none[4];
     __shared__ TeacherList lists[kRingLists];
-    __shared__ __align__(8) unsigned long long full[kRingChunks], done[kRingChunks];
+    __shared__ __align__(8) unsigned long long full[kRingSlots], done[kRingSlots];
     __shared__ int gave_up;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const size_t mine = (p.rows - blockIdx.x + gridDim.x - 1) / gridDim.x;
     if (threadIdx.x == 0) {
         gave_up = 0;
-        for (int b = 0; b < kRingChunks; ++b) { mbar_init(smem_u32(&full[b]), 1); mbar_init(smem_u32(&done[b]), kRingWarps); }
+        for (int b = 0; b < r.slots; ++b) { mbar_init(smem_u32(&full[b]), 1); mbar_init(smem_u32(&done[b]), kRingWarps + 1); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncthreads();
@@ -897,47 +913,57 @@ __global__ void __launch_bounds__(kRingThreads + 64, 1) distill_ring_kernel(Voca
         __syncwarp();
     };
     if (warp == kRingWarps + 1) {
-        auto bytes_of = [&](const Part& part, int c) { return (uint32_t)max(0, min(kChunkQuads, part.n4 - c * kChunkQuads)) * 16u; };
-        const size_t stages = mine * chunks;
-        size_t ahead = 0;                                         // next stage to load, chunk ahead_c of item ahead_item
-        size_t ahead_item = 0;
+        auto quads_of = [&](const Part& part, int c) { return max(0, min(r.chunk, part.n4 - c * r.chunk)); };
+        size_t ahead_item = 0;                                    // next to load: its chunk ahead_c
         int ahead_c = 0, slot_in = 0, slot_out = 0;
+        Part ahead = part_of(0);
         auto load = [&] {                                         // one lane
-            if (ahead >= stages) return;
-            const Part part = part_of(ahead_item);
-            const uint32_t n = bytes_of(part, ahead_c), bar = smem_u32(&full[slot_in]);
+            if (ahead_item >= mine) return;
+            const uint32_t n = quads_of(ahead, ahead_c) * 16u, bar = smem_u32(&full[slot_in]);
             mbar_expect_tx(bar, n);
-            if (n > 0) bulk_load(smem_u32(ring + slot_in * kChunkQuads), part.quads() + ahead_c * kChunkQuads, n, bar);
-            ++ahead;
-            if (++ahead_c == chunks) { ahead_c = 0; ++ahead_item; }
-            if (++slot_in == kRingChunks) slot_in = 0;
+            if (n > 0) bulk_load(smem_u32(ring + slot_in * r.chunk), ahead.quads() + ahead_c * r.chunk, n, bar);
+            if (++ahead_c == r.chunks) {
+                ahead_c = 0;
+                if (++ahead_item < mine) ahead = part_of(ahead_item);
+            }
+            if (++slot_in == r.slots) slot_in = 0;
         };
         if (lane == 0)
-            for (int i = 0; i < kRingChunks; ++i) load();
+            for (int i = 0; i < r.slots - 1; ++i) load();
         __syncwarp();
         uint32_t parity = 0;
         bool ok = true;
         auto write_behind = [&](size_t item) {
-            const float m = stat_m[item & 3], f = stat_f[item & 3];
-            if (f != 0.0f) list_write(list_warp.of(item), p.n_teacher, p.grad_logits + row_of(item) * p.stride, 0, p.cols, up, ProbGrad{m, p.c, f});
+            if (!ok || stat_none[item & 3]) return;
+            const TeacherList& list = list_warp.of(item);
+            float* g = p.grad_logits + row_of(item) * p.stride;
+            for (int i = lane; i < p.n_teacher; i += 32) {
+                const int id = list.id[i];
+                if (id >= 0 && id < p.cols) g[id] = list.g[i];
+            }
         };
         for (size_t item = 0; item < mine; ++item) {
             const Part part = part_of(item);
             float* g = p.grad_logits + row_of(item) * p.stride + part.head;
 #pragma unroll 1
-            for (int c = 0; c < chunks; ++c) {
+            for (int c = 0; c < r.chunks; ++c) {
                 if (ok && !mbar_wait_warp(smem_u32(&done[slot_out]), parity, &gave_up)) { ok = false; gone(); }
                 if (lane == 0 && ok) {
-                    const uint32_t n = bytes_of(part, c);
-                    if (n > 0) bulk_store(g + 4 * c * kChunkQuads, smem_u32(ring + slot_out * kChunkQuads), n);
+                    const int n = quads_of(part, c);
+                    if (n > 0) bulk_store(g + 4 * c * r.chunk, smem_u32(ring + slot_out * r.chunk), n * 16u);
                     bulk_end();
-                    asm volatile("cp.async.bulk.wait_group.read 2;" ::: "memory");
-                    if (item > 0 || c >= 2) load();               // to where the chunk before the last two has left
+                    asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+                    load();                                       // to where the chunk before this one was
                 }
-                if (++slot_out == kRingChunks) { slot_out = 0; parity ^= 1u; }
+                if (++slot_out == r.slots) { slot_out = 0; parity ^= 1u; }
             }
-            static_assert(kRingLeast >= 7, "what is pending is of this row");
-            if (lane == 0) asm volatile("cp.async.bulk.wait_group 7;" ::: "memory");
+            // what is pending then is of this row
+            if (lane == 0) {
+                if (r.chunks == 1) asm volatile("cp.async.bulk.wait_group 1;" ::: "memory");
+                else if (r.chunks == 2) asm volatile("cp.async.bulk.wait_group 2;" ::: "memory");
+                else if (r.chunks < 7) asm volatile("cp.async.bulk.wait_group 3;" ::: "memory");
+                else asm volatile("cp.async.bulk.wait_group 7;" ::: "memory");
+            }
             __syncwarp();
             if (item > 0) write_behind(item - 1);
         }
@@ -967,18 +993,19 @@ __global__ void __launch_bounds__(kRingThreads + 64, 1) distill_ring_kernel(Voca
         uint32_t at_parity = parity;
         if (!of_lists) {
 #pragma unroll 1
-            for (int c = 0; c < chunks; ++c) {
+            for (int c = 0; c < r.chunks; ++c) {
                 if (ok && !mbar_wait_warp(smem_u32(&full[at_slot]), at_parity, &gave_up)) { ok = false; gone(); }
-                float4 v[2];
+                const int n = min(r.chunk, part.n4 - c * r.chunk);
+                const float4* chunk = ring + at_slot * r.chunk;
+#pragma unroll 1
+                for (int i = threadIdx.x; i < n; i += 4 * kRingThreads) {
+                    float4 v[4];
 #pragma unroll
-                for (int u = 0; u < 2; ++u) v[u] = ring[at_slot * kChunkQuads + u * kRingThreads + threadIdx.x];
-                if ((c + 1) * kChunkQuads > part.n4) {
-#pragma unroll
-                    for (int u = 0; u < 2; ++u)
-                        if (c * kChunkQuads + u * kRingThreads + (int)threadIdx.x >= part.n4) v[u] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+                    for (int u = 0; u < 4; ++u)
+                        v[u] = i + u * kRingThreads < n ? chunk[i + u * kRingThreads] : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+                    run.quads(v, fmaxf(fmaxf(top_of(v[0]), top_of(v[1])), fmaxf(top_of(v[2]), top_of(v[3]))), p.c);
                 }
-                run.quads(v, fmaxf(top_of(v[0]), top_of(v[1])), p.c);
-                if (++at_slot == kRingChunks) { at_slot = 0; at_parity ^= 1u; }
+                if (++at_slot == r.slots) { at_slot = 0; at_parity ^= 1u; }
             }
             run.one(loose, p.c);
         }
@@ -996,28 +1023,32 @@ __global__ void __launch_bounds__(kRingThreads + 64, 1) distill_ring_kernel(Voca
         const TeacherList& list = list_warp.of(item);
         const float m = st.m, s = st.s, sg = gradient_sum(s, list.sum), f = sg == 0.0f ? 0.0f : up / sg;
         if (of_lists) {
+            if (!(sg == 0.0f)) list_gradients(list_warp.of(item), p.n_teacher, up, ProbGrad{m, p.c, f});
+            __syncwarp();
+            if (lane == 0)
+                for (int c = 0; c < r.chunks; ++c) {
+                    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&done[slot])) : "memory");
+                    if (++slot == r.slots) slot = 0;
+                }
             const float log_s = logf(s);
             const float loss = list_loss(list, p.n_teacher, [&](float v) { return s == 0.0f ? -INFINITY : (v - m) * p.inv_t - log_s; });
             list_result(p, list, row, m, s, loss);
             list_warp.ahead(item);
             continue;
         }
-        if (threadIdx.x == 0) { stat_m[item & 3] = m; stat_f[item & 3] = f; }
+        if (threadIdx.x == 0) stat_none[item & 3] = f == 0.0f;
         const ProbGrad value = {m, p.c, f};
         if (has_loose) p.grad_logits[row * p.stride + part.loose(threadIdx.x)] = f == 0.0f ? 0.0f : value(loose);
 #pragma unroll 1
-        for (int c = 0; c < chunks; ++c) {
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int i = u * kRingThreads + (int)threadIdx.x;
-                if (c * kChunkQuads + i >= part.n4) continue;
-                float4& at = ring[slot * kChunkQuads + i];
-                at = f == 0.0f ? make_float4(0.f, 0.f, 0.f, 0.f) : quad_of(at, value);
-            }
+        for (int c = 0; c < r.chunks; ++c) {
+            const int n = min(r.chunk, part.n4 - c * r.chunk);
+            float4* chunk = ring + slot * r.chunk;
+#pragma unroll 4
+            for (int i = threadIdx.x; i < n; i += kRingThreads) chunk[i] = f == 0.0f ? make_float4(0.f, 0.f, 0.f, 0.f) : quad_of(chunk[i], value);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&done[slot])) : "memory");
-            if (++slot == kRingChunks) { slot = 0; parity ^= 1u; }
+            if (++slot == r.slots) { slot = 0; parity ^= 1u; }
         }
     }
 }
@@ -1139,17 +1170,32 @@ cudaError_t launch_forward(VocabRows& p, int sm_count, cudaStream_t stream) {
     const cudaError_t e = smem <= 48 * 1024 - sizeof(RowShared) ? cudaSuccess : cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     return e != cudaSuccess ? e : launch_rows(kern, grid, kRowThreads, p.cluster, smem, stream, p);
 }
-// Rows of kRingLeast to kRingMost chunks, as many as keep all SMs busy, gradients on the logits' 16-byte boundaries.
+// Few chunks: each costs 1500 cycles of a row however small it is (4000 x 17800 in 2 / 4 / 8 of them 115 / 139 / 232 us).  But rows that come while one is at work need
+// room: two chunks more than a row has beside the one that goes out, where up to seven leave it (4096 x 32000 in 4 / 5 / 6 / 8: 194 / 185 / 206 / 240 us;
+// 4096 x 22000 in 2 / 3 / 4: 161 / 139 / 146), else as many as a row has (2500 x 40000 in 4 / 5 / 6: 158 / 157 / 169).  chunks = 0: too long.
+Ring ring_of(int cols) {
+    const int n4 = cols >> 2, all = (int)(kRingBytes / sizeof(float4));
+    Ring r = {n4, 1, kRingAhead + 1};
+    if (n4 * r.slots <= all) return r;
+    for (int room = 2; room >= 0; room -= 2)
+        for (r.chunks = 2; r.chunks <= (room ? 7 : kRingMost); ++r.chunks) {
+            r.chunk = (n4 + r.chunks - 1) / r.chunks;
+            r.slots = std::min((kRingAhead + 1) * r.chunks, all / r.chunk);
+            if (r.slots - 1 >= r.chunks + room) return r;
+        }
+    return {0, 0, 0};
+}
+// Rows of at least 11264 logits (3000 x 12000 with lists of 64: 86 us, twice out of L2 93; 3000 x 10000: 85 and 77; a row takes the list's warp 4 us however short it
+// is), as many as keep all SMs busy, gradients on the logits' 16-byte boundaries.
 bool ring_takes(const VocabRows& p, int sm_count, size_t max_smem) {
-    const size_t chunks = ((size_t)(p.cols >> 2) + kChunkQuads - 1) / kChunkQuads;
-    return chunks >= kRingLeast && chunks <= kRingMost && p.rows >= 2 * (size_t)sm_count && kRingBytes + kRingLists * sizeof(TeacherList) + 1024 <= max_smem &&
+    return p.cols >= 11264 && p.rows >= 2 * (size_t)sm_count && ring_of(p.cols).chunks > 0 && kRingBytes + kRingLists * sizeof(TeacherList) + 2048 <= max_smem &&
            ((reinterpret_cast<uintptr_t>(p.logits) ^ reinterpret_cast<uintptr_t>(p.grad_logits)) & 15) == 0;
 }
 cudaError_t launch_ring(VocabRows& p, int sm_count, cudaStream_t stream) {
-    const int chunks = ((p.cols >> 2) + kChunkQuads - 1) / kChunkQuads;
     const cudaError_t e = cudaFuncSetAttribute(distill_ring_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kRingBytes);
     if (e != cudaSuccess) return e;
-    return launch_chained(distill_ring_kernel, dim3((unsigned)(p.rows < (size_t)sm_count ? p.rows : sm_count)), dim3(kRingThreads + 64), kRingBytes, stream, p, chunks);
+    return launch_chained(distill_ring_kernel, dim3((unsigned)(p.rows < (size_t)sm_count ? p.rows : sm_count)), dim3(kRingThreads + 64), kRingBytes, stream, p,
+                          ring_of(p.cols));
 }
 void temperature_of(float t, float* c, float* inv_t) {
     *inv_t = 1.0f / t;
