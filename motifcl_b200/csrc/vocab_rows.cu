@@ -882,6 +882,17 @@ __device__ __forceinline__ void bulk_store(void* to, uint32_t from, uint32_t byt
     asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(to), "r"(from), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void bulk_end() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+// To the CTA `rank` of the cluster: a pair of values, counted by the barrier there.
+__device__ __forceinline__ void send_pair(const void* to, const void* bar, int rank, float a, float b) {
+    asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];" ::"r"(cluster_address(to, rank)), "f"(a), "f"(b),
+                 "r"(cluster_address(bar, rank)) : "memory");
+}
+// A completed phase once more, for what other CTAs have written.
+__device__ __forceinline__ void cluster_acquire(uint32_t bar, uint32_t parity) {
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%0], %1;\n\t}" ::"r"(bar), "r"(parity) : "memory");
+}
+// CLUSTER: a CTA has a part of a row; the parts' statistics cross the cluster once a row, to barriers that count them.
+template <bool CLUSTER>
 __global__ void __launch_bounds__(kRingThreads + 64, 1) distill_ring_kernel(VocabRows p, Ring r) {
     grid_release();
     extern __shared__ __align__(16) unsigned char dynamic[];
@@ -890,18 +901,25 @@ __global__ void __launch_bounds__(kRingThreads + 64, 1) distill_ring_kernel(Voca
     __shared__ bool stat_none[4];
     __shared__ TeacherList lists[kRingLists];
     __shared__ __align__(8) unsigned long long full[kRingSlots], done[kRingSlots];
+    __shared__ __align__(8) float2 parts[2][kMaxCluster];
+    __shared__ __align__(8) unsigned long long crossed[2];
     __shared__ int gave_up;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const size_t mine = (p.rows - blockIdx.x + gridDim.x - 1) / gridDim.x;
+    const int ranks = CLUSTER ? p.cluster : 1, rank = CLUSTER ? (int)(blockIdx.x % ranks) : 0;
+    const int per = ((p.cols + ranks - 1) / ranks + 3) & ~3;
+    const int c0 = rank * per, cn = min(p.cols, c0 + per) - c0;
+    const size_t first = blockIdx.x / ranks, step = gridDim.x / ranks, mine = (p.rows - first + step - 1) / step;
     if (threadIdx.x == 0) {
         gave_up = 0;
         for (int b = 0; b < r.slots; ++b) { mbar_init(smem_u32(&full[b]), 1); mbar_init(smem_u32(&done[b]), kRingWarps + 1); }
+        for (int b = 0; b < 2; ++b) mbar_init(smem_u32(&crossed[b]), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncthreads();
+    if (CLUSTER) { cluster_arrive(); cluster_wait(); }            // the others' barriers are there
     grid_wait();
-    auto row_of = [&](size_t i) { return blockIdx.x + i * gridDim.x; };
-    auto part_of = [&](size_t i) { return Part(p.logits + row_of(i) * p.stride, p.cols); };
+    auto row_of = [&](size_t i) { return first + i * step; };
+    auto part_of = [&](size_t i) { return Part(p.logits + row_of(i) * p.stride + c0, cn); };
     ListWarp<kRingLists, VocabRows, decltype(row_of)> list_warp = {lists, p, mine, row_of};
     const float up = load_behind(p.grad_out) * p.inv_t / (float)p.rows;
     // Where a wait runs out the call's results are void: the error word says so, nobody waits any more, and every loop runs to its end.
@@ -936,15 +954,15 @@ __global__ void __launch_bounds__(kRingThreads + 64, 1) distill_ring_kernel(Voca
         auto write_behind = [&](size_t item) {
             if (!ok || stat_none[item & 3]) return;
             const TeacherList& list = list_warp.of(item);
-            float* g = p.grad_logits + row_of(item) * p.stride;
+            float* g = p.grad_logits + row_of(item) * p.stride + c0;
             for (int i = lane; i < p.n_teacher; i += 32) {
                 const int id = list.id[i];
-                if (id >= 0 && id < p.cols) g[id] = list.g[i];
+                if (id >= c0 && id - c0 < cn) g[id - c0] = list.g[i];
             }
         };
         for (size_t item = 0; item < mine; ++item) {
             const Part part = part_of(item);
-            float* g = p.grad_logits + row_of(item) * p.stride + part.head;
+            float* g = p.grad_logits + row_of(item) * p.stride + c0 + part.head;
 #pragma unroll 1
             for (int c = 0; c < r.chunks; ++c) {
                 if (ok && !mbar_wait_warp(smem_u32(&done[slot_out]), parity, &gave_up)) { ok = false; gone(); }
@@ -975,6 +993,7 @@ __global__ void __launch_bounds__(kRingThreads + 64, 1) distill_ring_kernel(Voca
             const unsigned long long t0 = clock64();
             while (clock64() - t0 < 2000000ull) {}
         }
+        if (CLUSTER) { __syncwarp(); cluster_arrive(); cluster_wait(); }
         return;
     }
     const bool of_lists = warp == kRingWarps;
@@ -1019,6 +1038,20 @@ __global__ void __launch_bounds__(kRingThreads + 64, 1) distill_ring_kernel(Voca
         st.m = wm[turn][lane & (kRingWarps - 1)];
         st.s = ws[turn][lane & (kRingWarps - 1)];
         st.join<kRingWarps>(p.c);
+        if (CLUSTER) {
+            if (warp == 0) {
+                if (lane == 0) mbar_expect_tx(smem_u32(&crossed[turn]), ranks * 8);
+                if (lane < ranks) send_pair(&parts[turn][rank], &crossed[turn], lane, st.m, st.s);
+            }
+            const uint32_t phase = (uint32_t)(item >> 1) & 1u;
+            if (ok && !mbar_wait_warp(smem_u32(&crossed[turn]), phase, &gave_up)) { ok = false; gone(); }
+            if (ok) cluster_acquire(smem_u32(&crossed[turn]), phase);
+            st = Stats<false>();
+            if (lane < ranks) { st.m = parts[turn][lane].x; st.s = parts[turn][lane].y; }
+            st.join<kMaxCluster>(p.c);
+            st.m = __shfl_sync(0xffffffffu, st.m, 0);
+            st.s = __shfl_sync(0xffffffffu, st.s, 0);
+        }
         // an empty list or an empty row has no gradient; a list that is not a number has none that is one
         const TeacherList& list = list_warp.of(item);
         const float m = st.m, s = st.s, sg = gradient_sum(s, list.sum), f = sg == 0.0f ? 0.0f : up / sg;
@@ -1032,13 +1065,13 @@ __global__ void __launch_bounds__(kRingThreads + 64, 1) distill_ring_kernel(Voca
                 }
             const float log_s = logf(s);
             const float loss = list_loss(list, p.n_teacher, [&](float v) { return s == 0.0f ? -INFINITY : (v - m) * p.inv_t - log_s; });
-            list_result(p, list, row, m, s, loss);
+            if (rank == 0) list_result(p, list, row, m, s, loss);
             list_warp.ahead(item);
             continue;
         }
         if (threadIdx.x == 0) stat_none[item & 3] = f == 0.0f;
         const ProbGrad value = {m, p.c, f};
-        if (has_loose) p.grad_logits[row * p.stride + part.loose(threadIdx.x)] = f == 0.0f ? 0.0f : value(loose);
+        if (has_loose) p.grad_logits[row * p.stride + c0 + part.loose(threadIdx.x)] = f == 0.0f ? 0.0f : value(loose);
 #pragma unroll 1
         for (int c = 0; c < r.chunks; ++c) {
             const int n = min(r.chunk, part.n4 - c * r.chunk);
@@ -1051,6 +1084,7 @@ __global__ void __launch_bounds__(kRingThreads + 64, 1) distill_ring_kernel(Voca
             if (++slot == r.slots) { slot = 0; parity ^= 1u; }
         }
     }
+    if (CLUSTER) { __syncwarp(); cluster_arrive(); cluster_wait(); }      // nothing more comes to this CTA's shared memory
 }
 
 // ---- gradients from kept statistics ------------------------------------------------------------------------------------
@@ -1136,8 +1170,8 @@ __global__ void __launch_bounds__(kRowThreads, 4) vocab_grad_kernel(VocabGrad p)
 }
 
 // Attributes of a launch: overlapping with the one before it, and the CTAs of a row as a cluster.
-template <class P>
-cudaError_t launch_rows(void (*kern)(P), unsigned grid, int threads, int cluster, size_t smem, cudaStream_t stream, const P& p) {
+template <class... P>
+cudaError_t launch_rows(void (*kern)(P...), unsigned grid, int threads, int cluster, size_t smem, cudaStream_t stream, const P&... p) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid); cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = smem; cfg.stream = stream;
     cudaLaunchAttribute at[2];
@@ -1146,7 +1180,7 @@ cudaError_t launch_rows(void (*kern)(P), unsigned grid, int threads, int cluster
     at[1].id = cudaLaunchAttributeClusterDimension;
     at[1].val.clusterDim.x = cluster; at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
     cfg.attrs = at; cfg.numAttrs = cluster > 1 ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, kern, p);
+    return cudaLaunchKernelEx(&cfg, kern, p...);
 }
 // CTAs of a row: as many as leave none of the SMs idle, with 2048 logits each at least (one row of 32000: 6.8 us by eight, 16 rows 7.5)
 int row_cluster(size_t rows, int cols, int sm_count) {
@@ -1187,15 +1221,32 @@ Ring ring_of(int cols) {
 }
 // Rows of at least 11264 logits (3000 x 12000 with lists of 64: 86 us, twice out of L2 93; 3000 x 10000: 85 and 77; a row takes the list's warp 4 us however short it
 // is), as many as keep all SMs busy, gradients on the logits' 16-byte boundaries.
-bool ring_takes(const VocabRows& p, int sm_count, size_t max_smem) {
-    return p.cols >= 11264 && p.rows >= 2 * (size_t)sm_count && ring_of(p.cols).chunks > 0 && kRingBytes + kRingLists * sizeof(TeacherList) + 2048 <= max_smem &&
+// Longer ones by the CTAs of a cluster.
+bool ring_takes(VocabRows& p, int sm_count, size_t max_smem) {
+    const auto part = [&] { return ((p.cols + p.cluster - 1) / p.cluster + 3) & ~3; };
+    for (p.cluster = 1; ring_of(part()).chunks == 0; p.cluster *= 2)
+        if (p.cluster == kMaxCluster) return false;
+    return p.cols >= 11264 && p.rows * p.cluster >= 2 * (size_t)sm_count && kRingBytes + kRingLists * sizeof(TeacherList) + 2048 <= max_smem &&
            ((reinterpret_cast<uintptr_t>(p.logits) ^ reinterpret_cast<uintptr_t>(p.grad_logits)) & 15) == 0;
 }
 cudaError_t launch_ring(VocabRows& p, int sm_count, cudaStream_t stream) {
-    const cudaError_t e = cudaFuncSetAttribute(distill_ring_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kRingBytes);
+    const auto kern = p.cluster > 1 ? distill_ring_kernel<true> : distill_ring_kernel<false>;
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kRingBytes);
     if (e != cudaSuccess) return e;
-    return launch_chained(distill_ring_kernel, dim3((unsigned)(p.rows < (size_t)sm_count ? p.rows : sm_count)), dim3(kRingThreads + 64), kRingBytes, stream, p,
-                          ring_of(p.cols));
+    size_t at_once = sm_count;
+    if (p.cluster > 1) {                              // as many as run at once: those of 4 or 8 do not fill every part of the GPU
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(p.cluster); cfg.blockDim = dim3(kRingThreads + 64); cfg.dynamicSmemBytes = kRingBytes;
+        cudaLaunchAttribute at;
+        at.id = cudaLaunchAttributeClusterDimension;
+        at.val.clusterDim.x = p.cluster; at.val.clusterDim.y = at.val.clusterDim.z = 1;
+        cfg.attrs = &at; cfg.numAttrs = 1;
+        int n = 0;
+        if ((e = cudaOccupancyMaxActiveClusters(&n, kern, &cfg)) != cudaSuccess) return e;
+        at_once = n > 0 ? n : 1;
+    }
+    const Ring r = ring_of(((p.cols + p.cluster - 1) / p.cluster + 3) & ~3);
+    return launch_rows(kern, (unsigned)((p.rows < at_once ? p.rows : at_once) * p.cluster), kRingThreads + 64, p.cluster, kRingBytes, stream, p, r);
 }
 void temperature_of(float t, float* c, float* inv_t) {
     *inv_t = 1.0f / t;

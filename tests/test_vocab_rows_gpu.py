@@ -427,6 +427,29 @@ def test_distillation(ctx, R, V, K, pad, offset, T, form):
     near(got, grad, tol_g, "gradient")
 
 
+# rows in the ring of chunks: three whole ones, in two to seven chunks, as long as there is room for, and in parts over two, four and eight CTAs;
+# every row at another alignment where the pad is odd
+@pytest.mark.parametrize("R,V,K,pad,offset,T", [(700, 11264, 20, 0, 0, 1.0), (301, 13001, 128, 1, 0, 2.0), (500, 17749, 9, 0, 2, 1.0), (450, 20003, 64, 2, 1, 0.8),
+                                              (310, 22001, 33, 0, 0, 1.0), (300, 28004, 5, 1, 3, 1.0), (299, 36000, 64, 0, 0, 1.5), (298, 40001, 7, 0, 1, 1.0),
+                                              (297, 49152, 16, 0, 0, 1.0), (310, 49157, 64, 0, 1, 1.0), (170, 70001, 100, 1, 0, 2.0), (160, 128256, 64, 0, 0, 1.0),
+                                              (76, 150003, 11, 2, 3, 1.0), (45, 262144, 8, 0, 0, 1.0)])
+@pytest.mark.parametrize("form", ["one call", "in place"])
+def test_distillation_of_long_rows(ctx, R, V, K, pad, offset, T, form):
+    x, stride = make_logits(R, V, pad, offset, seed=17)
+    ids, a = make_teacher(R, V, K, 6)
+    ids[1, K // 2:] = -1
+    ids[2] = V
+    ids[3, 1:] = ids[3, 0]                                          # one token K times
+    ids[4, :4] = torch.tensor([0, V - 1, 1, V - 2])                 # at the ends, outside whole quads
+    x[5] = NEG
+    x[6, V // 4:] = NEG                                             # CTAs of which nothing is left
+    x[7] = LOWEST
+    losses, tol_l, grad, tol_g = distill_ref(x, ids, a, T, 0.5)
+    part, out, got = run_distill(ctx, x, stride, ids, a, T, 0.5, form)
+    near(part, losses, tol_l, "losses")
+    near(got, grad, tol_g, "gradient")
+
+
 @pytest.mark.parametrize("form", FORMS)
 @pytest.mark.parametrize("R,V", [(16, 500), (16, 40000), (320, 26000)])
 def test_distillation_lists_and_rows_that_go_wrong(ctx, R, V, form):
@@ -478,7 +501,7 @@ def test_distillation_lists_longer_than_a_warp(ctx, K, form):
 
 
 @pytest.mark.parametrize("form", ["one call", "split"])
-@pytest.mark.parametrize("R,V", [(7, 3000), (300, 25001)])
+@pytest.mark.parametrize("R,V", [(7, 3000), (300, 25001), (160, 60001)])
 def test_distillation_of_rows_with_nan(ctx, R, V, form):
     K = 5
     x, stride = make_logits(R, V, seed=12)
