@@ -859,11 +859,14 @@ __global__ void __launch_bounds__(kRowThreads, 4) vocab_rows_kernel(VocabRows p)
 
 // ---- loss and gradient of long rows in one pass ---------------------------------------------------------------------------
 // A row comes to shared memory once, in chunks by bulk copies, becomes its gradient there, and goes out by bulk copies: a ring of chunks in which the
-// next row comes while this one is at work and the one before goes.  The threads themselves neither load nor store: behind their own stores all
-// of an SM's memory instructions, those on shared memory among them, waited two thirds of the time.  4096 x 32000 with lists of 64: 191 us, 85 % of the copy's
-// rate; the row a second time out of L2 300 us with four rows on an SM, of which L2 keeps none, 325 with three, 398 with two, 549 with one; a row in shared memory
-// with the threads' own copies and stores 219.
-// Two more warps: one has the teacher's lists and forms the losses; one issues the copies and writes the listed tokens' gradients a row behind.
+// next rows come while this one is at work and the one before goes.  The threads themselves neither load nor store: behind their own stores all
+// of an SM's memory instructions, those on shared memory among them, waited two thirds of the time.  Bound by memory, read and write.  4096 x 32000 with lists of
+// 64: 184 us, 88 % of the copy's rate, 5000 x 20000 148 us (84 %), 1000 x 128256 222 us (72 %); the rows of 32000 a second time out of L2 300 us with four rows on an
+// SM, of which L2 keeps none, 325 with three, 398 with two, 549 with one; a row in shared memory with the threads' own copies and stores 219.
+// Two more warps: one has the teacher's lists, forms the losses and the listed tokens' gradients; one issues the copies and writes those gradients a row behind,
+// when the bulk copies of their row are done.
+// Nothing may be ahead of the copying warp by more than its ring: a row's statistics need all of its chunks, of which there are kRingAhead rows beside the one
+// that goes out, so that while that is row i, rows up to i + 2 have statistics and lists up to row i + 4 are fetched; of row i - 1 the list is still needed.
 constexpr int kRingThreads = 512;      // that work on rows
 constexpr int kRingWarps = kRingThreads / 32;
 constexpr size_t kRingBytes = 208 * 1024;
@@ -1221,10 +1224,11 @@ Ring ring_of(int cols) {
 }
 // Rows of at least 11264 logits (3000 x 12000 with lists of 64: 86 us, twice out of L2 93; 3000 x 10000: 85 and 77; a row takes the list's warp 4 us however short it
 // is), as many as keep all SMs busy, gradients on the logits' 16-byte boundaries.
-// Longer ones by the CTAs of a cluster.
+// Longer ones by as many CTAs as hold a row: more of them are more clusters' seams and fewer clusters that fit the GPU (1000 x 128256 by 3 / 4 / 6: 222 / 240 / 252 us,
+// 400 x 262144 by 6 / 8: 193 / 223, 2000 x 60000 by 2 / 3: 190 / 223; twice out of L2 298, 256 and 285).
 bool ring_takes(VocabRows& p, int sm_count, size_t max_smem) {
     const auto part = [&] { return ((p.cols + p.cluster - 1) / p.cluster + 3) & ~3; };
-    for (p.cluster = 1; ring_of(part()).chunks == 0; p.cluster *= 2)
+    for (p.cluster = 1; ring_of(part()).chunks == 0; ++p.cluster)
         if (p.cluster == kMaxCluster) return false;
     return p.cols >= 11264 && p.rows * p.cluster >= 2 * (size_t)sm_count && kRingBytes + kRingLists * sizeof(TeacherList) + 2048 <= max_smem &&
            ((reinterpret_cast<uintptr_t>(p.logits) ^ reinterpret_cast<uintptr_t>(p.grad_logits)) & 15) == 0;
@@ -1234,7 +1238,7 @@ cudaError_t launch_ring(VocabRows& p, int sm_count, cudaStream_t stream) {
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kRingBytes);
     if (e != cudaSuccess) return e;
     size_t at_once = sm_count;
-    if (p.cluster > 1) {                              // as many as run at once: those of 4 or 8 do not fill every part of the GPU
+    if (p.cluster > 1) {                              // as many as run at once: large ones do not fill every part of the GPU
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(p.cluster); cfg.blockDim = dim3(kRingThreads + 64); cfg.dynamicSmemBytes = kRingBytes;
         cudaLaunchAttribute at;
