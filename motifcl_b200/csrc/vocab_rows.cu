@@ -1185,14 +1185,19 @@ cudaError_t launch_rows(void (*kern)(P...), unsigned grid, int threads, int clus
     cfg.attrs = at; cfg.numAttrs = cluster > 1 ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kern, p...);
 }
-// CTAs of a row: as many as leave none of the SMs idle, with 2048 logits each at least (one row of 32000: 6.8 us by eight, 16 rows 7.5)
-int row_cluster(size_t rows, int cols, int sm_count) {
+// CTAs of a row: as many as leave none of the SMs idle, with 2048 logits each at least (one row of 32000: 6.8 us by eight, 16 rows 7.5).  Up to four on an SM (three
+// with a selection's shared memory) where a CTA's part stays long enough to pay for the cluster's seam.  One / two CTAs: 200 x 128256 statistics 23 / 20 us, with 20 tops
+// 33 / 26, lists' losses 27 / 22, but 150 x 50003 statistics 10.3 / 11.1; the gradient, a second pass over what L2 holds of a row, gains from shorter
+// parts on: 150 x 24000 19 / 17.6, 200 x 14000 14.4 / 12.8.
+int row_cluster(const VocabRows& p, int sm_count) {
+    const size_t most = p.n_top ? 3 : 4;
+    const int least = p.grad_logits ? 6144 : p.n_top || p.n_teacher ? 24576 : 30720;
     int n = 1;
-    while (n < kMaxCluster && rows * 2 * n <= 2 * (size_t)sm_count && cols / (2 * n) >= 2048) n *= 2;
+    while (n < kMaxCluster && ((p.rows * 2 * n <= 2 * (size_t)sm_count && p.cols / (2 * n) >= 2048) || (p.rows * 2 * n <= most * sm_count && p.cols / (2 * n) >= least))) n *= 2;
     return n;
 }
 cudaError_t launch_forward(VocabRows& p, int sm_count, cudaStream_t stream) {
-    p.cluster = row_cluster(p.rows, p.cols, sm_count);
+    p.cluster = row_cluster(p, sm_count);
     // Bounds after 1, 2, 4, 8, ... steps, between two of which there are as many hits again; after 1 and 2 only where a barrier and a bound are more than the
     // hits they save.  All of them / two, k = 20: 4096 x 32000 (8 steps) 112 / 110 us, 2000 x 50003 82 / 86, 600 x 128256 69 / 122; k = 64:
     // 147 / 139, 99 / 138, 76 / 140; k = 128, 4096 x 32000: 231 / 302, as two leave more than kHits.
@@ -1230,6 +1235,8 @@ bool ring_takes(VocabRows& p, int sm_count, size_t max_smem) {
     const auto part = [&] { return ((p.cols + p.cluster - 1) / p.cluster + 3) & ~3; };
     for (p.cluster = 1; ring_of(part()).chunks == 0; ++p.cluster)
         if (p.cluster == kMaxCluster) return false;
+    // few rows: in parts of no fewer than 11264 (200 x 32000 by one CTA 25 us, by two, twice out of L2, 21.6, by two here 18.2)
+    while (p.rows * p.cluster < 2 * (size_t)sm_count && p.cluster < kMaxCluster && p.cols / (p.cluster + 1) >= 11264) ++p.cluster;
     return p.cols >= 11264 && p.rows * p.cluster >= 2 * (size_t)sm_count && kRingBytes + kRingLists * sizeof(TeacherList) + 2048 <= max_smem &&
            ((reinterpret_cast<uintptr_t>(p.logits) ^ reinterpret_cast<uintptr_t>(p.grad_logits)) & 15) == 0;
 }

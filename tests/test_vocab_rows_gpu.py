@@ -141,6 +141,8 @@ def check_logprobs(ctx, x, stride, k, T, tokens):
     (40, 32000, 64, 0, 64, 0.3),
     (2, 150001, 0, 0, 50, 1.0),
     (300, 32000, 0, 0, 1, 1.0),
+    (190, 60003, 1, 0, 20, 1.0),          # two CTAs a row, three on an SM
+    (110, 128256, 0, 0, 128, 1.0),
 ])
 def test_token_logprobs(ctx, R, V, pad, offset, k, T):
     x, stride = make_logits(R, V, pad, offset, seed=1)
@@ -432,7 +434,8 @@ def test_distillation(ctx, R, V, K, pad, offset, T, form):
 @pytest.mark.parametrize("R,V,K,pad,offset,T", [(700, 11264, 20, 0, 0, 1.0), (301, 13001, 128, 1, 0, 2.0), (500, 17749, 9, 0, 2, 1.0), (450, 20003, 64, 2, 1, 0.8),
                                               (310, 22001, 33, 0, 0, 1.0), (300, 28004, 5, 1, 3, 1.0), (299, 36000, 64, 0, 0, 1.5), (298, 40001, 7, 0, 1, 1.0),
                                               (297, 49152, 16, 0, 0, 1.0), (310, 49157, 64, 0, 1, 1.0), (170, 70001, 100, 1, 0, 2.0), (160, 128256, 64, 0, 0, 1.0),
-                                              (76, 150003, 11, 2, 3, 1.0), (45, 262144, 8, 0, 0, 1.0)])
+                                              (76, 150003, 11, 2, 3, 1.0), (45, 262144, 8, 0, 0, 1.0), (200, 24001, 20, 3, 0, 1.0), (110, 50003, 64, 0, 0, 1.0),
+                                              (100, 24001, 20, 3, 0, 1.0)])
 @pytest.mark.parametrize("form", ["one call", "in place"])
 def test_distillation_of_long_rows(ctx, R, V, K, pad, offset, T, form):
     x, stride = make_logits(R, V, pad, offset, seed=17)
