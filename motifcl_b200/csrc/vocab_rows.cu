@@ -19,6 +19,7 @@
 #include <cfloat>
 #include <climits>
 #include <cmath>
+#include <type_traits>
 
 namespace mcl {
 namespace {
@@ -1108,6 +1109,33 @@ struct VocabGrad {
     float* grad_logits;
 };
 
+// What a row's gradient is formed from.
+struct Terms {
+    float k0, k1, up;
+    int token;                         // -1: none
+    bool none;                         // all of the gradient is 0
+};
+template <bool DISTILL>
+__device__ __forceinline__ Terms grad_terms(const VocabGrad& p, size_t row, float m, float s) {
+    Terms t = {0.0f, 0.0f, 0.0f, -1, s == 0.0f};
+    if (DISTILL) {
+        t.up = load_behind(p.grad_out) * p.inv_t / (float)p.rows;
+        t.k0 = t.up / s;
+        return t;
+    }
+    float h = 0.0f, H = 0.0f;
+    if (p.grad_logprobs != nullptr) {
+        t.token = load_behind(p.tokens + row);
+        if (t.token < 0 || t.token >= p.cols) t.token = -1;
+        else t.up = load_behind(p.grad_logprobs + row) * p.inv_t;
+    }
+    if (p.grad_entropy != nullptr) { h = load_behind(p.grad_entropy + row) * p.inv_t; H = load_behind(p.entropy + row); }
+    t.none = t.none || (t.up == 0.0f && h == 0.0f);
+    t.k0 = -(t.up + (h == 0.0f ? 0.0f : h * (H - logf(s)))) / s;
+    t.k1 = -h * kLn2 / s;
+    return t;
+}
+
 // dx_c = e_c (k0 + k1 d_c) + (what the named tokens add), with e_c = 2^((x_c - m) c): p_c enters through 1 / s in k0 and k1.
 // Bound by memory, read and write: 4096 x 32000 in 161 us, a copy's rate; from lists of 64 176 us, as a CTA's writing ends in one warp's work.
 // DISTILL: the first warp has an item's list on its way from the start, and takes the listed tokens' probabilities off when the rest is written.
@@ -1129,35 +1157,19 @@ __global__ void __launch_bounds__(kRowThreads, 4) vocab_grad_kernel(VocabGrad p)
         load_step(part, q, 0, v);
         const float loose = (int)threadIdx.x < part.n - 4 * part.n4 ? load_behind(part.p + part.loose(threadIdx.x)) : 0.0f;
         const float m = load_behind(p.row_stats + 2 * row), s = load_behind(p.row_stats + 2 * row + 1);
-        float k0 = 0.0f, k1 = 0.0f, up = 0.0f, x_token = 0.0f;
-        int token = -1;
-        bool none = s == 0.0f;
-        if (DISTILL) {
-            if (warp == 0) { list_fetch(list, p, row); copies_end(); }
-            up = load_behind(p.grad_out) * p.inv_t / (float)p.rows;
-            k0 = up / s;
-        } else {
-            float h = 0.0f, H = 0.0f;
-            if (p.grad_logprobs != nullptr) {
-                token = load_behind(p.tokens + row);
-                if (token < 0 || token >= p.cols) token = -1;
-                else {
-                    up = load_behind(p.grad_logprobs + row) * p.inv_t;
-                    if (threadIdx.x == 0) x_token = load_behind(x + token);
-                }
-            }
-            if (p.grad_entropy != nullptr) { h = load_behind(p.grad_entropy + row) * p.inv_t; H = load_behind(p.entropy + row); }
-            none = none || (up == 0.0f && h == 0.0f);
-            k0 = -(up + (h == 0.0f ? 0.0f : h * (H - logf(s)))) / s;
-            k1 = -h * kLn2 / s;
+        if (DISTILL && warp == 0) { list_fetch(list, p, row); copies_end(); }
+        const Terms terms = grad_terms<DISTILL>(p, row, m, s);
+        float x_token = 0.0f;
+        if (!DISTILL) {
+            if (threadIdx.x == 0 && terms.token >= 0) x_token = load_behind(x + terms.token);
             __syncthreads();        // the token's logit is read before any of the row is written (grad_logits may be logits); other tiles' are not used
         }
-        const EntropyGrad with_entropy = {m, p.c, k0, k1};
-        if (DISTILL) write_part<kRowThreads>(part, q, g, v, loose, none, ProbGrad{m, p.c, k0});
-        else write_part<kRowThreads>(part, q, g, v, loose, none, with_entropy);
+        const EntropyGrad with_entropy = {m, p.c, terms.k0, terms.k1};
+        if (DISTILL) write_part<kRowThreads>(part, q, g, v, loose, terms.none, ProbGrad{m, p.c, terms.k0});
+        else write_part<kRowThreads>(part, q, g, v, loose, terms.none, with_entropy);
         __syncthreads();
-        if (!DISTILL && threadIdx.x == 0 && !none && token >= c0 && token < c0 + cn) g[token - c0] = with_entropy(x_token) + up;
-        if (DISTILL && warp == 0 && !none) {
+        if (!DISTILL && threadIdx.x == 0 && !terms.none && terms.token >= c0 && terms.token < c0 + cn) g[terms.token - c0] = with_entropy(x_token) + terms.up;
+        if (DISTILL && warp == 0 && !terms.none) {
             copies_wait<0>();
             __syncwarp();
             for (int i = lane; i < p.n_teacher; i += 32)
@@ -1166,8 +1178,146 @@ __global__ void __launch_bounds__(kRowThreads, 4) vocab_grad_kernel(VocabGrad p)
             const bool twice = list_twice(list, p);
             if (lane == 0) list.twice = twice;
             __syncwarp();
-            each_listed(list, p.n_teacher, c0, cn, [&](int, int at, float t) { g[at] -= t * up; });      // p is there
+            each_listed(list, p.n_teacher, c0, cn, [&](int, int at, float t) { g[at] -= t * terms.up; });      // p is there
             __syncwarp();                                         // before the next item's list comes
+        }
+    }
+}
+
+// ---- short rows: a warp for each, which holds it in registers ----------------------------------------------------------------
+// Up to 128 J logits, J quads a lane; no barrier, the largest logit is known before the first exponential, and 16 and more rows of an SM are on their way.  What a CTA
+// spends on a row beside its logits, 2.4 us, is more than short rows take: 11000 x 1000 by CTAs / by warps: statistics 47 / 11 us, their gradient 40 / 14, lists' loss
+// 54 / 17, loss and gradient 83 / 27 us; 40000 x 2000: 167 / 54 (92 % of the copy's rate), 161 / 101 (98 %), 177 / 94, 318 / 118 (84 %).
+template <int J>
+struct ShortRow {
+    Part part;
+    float4 v[J];
+    float loose;                       // outside the quads: one of the first lanes each
+    __device__ __forceinline__ ShortRow(const float* row, int n) : part(row, n), loose(-INFINITY) {
+        const int lane = threadIdx.x & 31;
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            v[j] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+            if (lane + 32 * j < part.n4) v[j] = load_behind(part.quads() + lane + 32 * j);
+        }
+        if (lane < part.n - 4 * part.n4) loose = load_behind(part.p + part.loose(lane));
+    }
+    template <bool ENTROPY>
+    __device__ __forceinline__ Stats<ENTROPY> stats(float c) const {
+        float top = fmaxf(-FLT_MAX, loose);
+#pragma unroll
+        for (int j = 0; j < J; ++j) top = fmaxf(top, top_of(v[j]));
+        top = warp_top(top);
+        Running<ENTROPY> run;
+        run.m = top;
+        run.minus_m = pair_of(-top, -top);
+#pragma unroll
+        for (int j = 0; j < J; ++j) { run.terms(pair_of(v[j].x, v[j].y), c); run.terms(pair_of(v[j].z, v[j].w), c); }
+        run.terms(pair_of(loose, -INFINITY), c);
+        Stats<ENTROPY> st = run.sums();
+        st.s = warp_add(st.s);
+        if (ENTROPY) st.a = warp_add(st.a);
+        return st;
+    }
+    template <class F>
+    __device__ __forceinline__ void write(float* g, bool none, F f) const {
+        const int lane = threadIdx.x & 31;
+        const bool vec = ((reinterpret_cast<uintptr_t>(g) ^ reinterpret_cast<uintptr_t>(part.p)) & 15) == 0;
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            if (lane + 32 * j >= part.n4) continue;
+            float* to = g + part.head + 4 * (lane + 32 * j);
+            const float4 o = none ? make_float4(0.f, 0.f, 0.f, 0.f) : quad_of(v[j], f);
+            if (vec) *reinterpret_cast<float4*>(to) = o;
+            else { to[0] = o.x; to[1] = o.y; to[2] = o.z; to[3] = o.w; }
+        }
+        if (lane < part.n - 4 * part.n4) g[part.loose(lane)] = none ? 0.0f : f(loose);
+    }
+};
+// A row's list and the logits at its ids (where p has logits to look at), by the warp that has the row.
+template <class P>
+__device__ __forceinline__ void list_ready(TeacherList& l, const P& p, size_t row) {
+    copies_wait<0>();
+    __syncwarp();
+    list_gather(l, p, row);
+    copies_end();
+    __syncwarp();
+    list_terms(l, p);
+    const bool twice = list_twice(l, p);
+    if ((threadIdx.x & 31) == 0) l.twice = twice;
+    copies_wait<0>();
+    __syncwarp();
+}
+template <int J, bool ENTROPY, RowWork WORK>
+__global__ void __launch_bounds__(kRowThreads) short_rows_kernel(VocabRows p) {
+    constexpr bool DISTILL = WORK == kList || WORK == kGrad, GRAD = WORK == kGrad;
+    grid_release();
+    grid_wait();
+    __shared__ TeacherList lists[DISTILL ? kRowWarps : 1];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    TeacherList& list = lists[DISTILL ? warp : 0];
+    const float up = GRAD ? load_behind(p.grad_out) * p.inv_t / (float)p.rows : 0.0f;
+    for (size_t row = (size_t)blockIdx.x * kRowWarps + warp; row < p.rows; row += (size_t)gridDim.x * kRowWarps) {
+        const float* x = p.logits + row * p.stride;
+        if (DISTILL) { list_fetch(list, p, row); copies_end(); }
+        int token = -1;
+        float x_token = 0.0f;
+        if (!DISTILL && p.tokens != nullptr && lane == 0) {
+            token = load_behind(p.tokens + row);
+            if (token < 0 || token >= p.cols) token = -1;
+            else x_token = load_behind(x + token);
+        }
+        const ShortRow<J> r(x, p.cols);
+        const Stats<ENTROPY> st = r.template stats<ENTROPY>(p.c);
+        const float m = st.m, s = st.s, log_s = logf(s);
+        auto log_prob = [&](float value) { return s == 0.0f ? -INFINITY : (value - m) * p.inv_t - log_s; };      // s == 0: nothing is left of the row
+        if (!DISTILL && lane == 0) {
+            if (p.row_stats != nullptr) { p.row_stats[2 * row] = m; p.row_stats[2 * row + 1] = s; }
+            if (p.logprobs != nullptr) p.logprobs[row] = token < 0 ? 0.0f : log_prob(x_token);
+            if (ENTROPY) p.entropy[row] = s == 0.0f ? 0.0f : log_s - st.a / s * kLn2;
+        }
+        if (DISTILL) {
+            list_ready(list, p, row);
+            list_result(p, list, row, m, s, list_loss(list, p.n_teacher, log_prob));
+            if (GRAD) {
+                const float sg = gradient_sum(s, list.sum);
+                const ProbGrad value = {m, p.c, up / sg};
+                r.write(p.grad_logits + row * p.stride, sg == 0.0f, value);
+                __syncwarp();
+                if (!(sg == 0.0f)) list_write(list, p.n_teacher, p.grad_logits + row * p.stride, 0, p.cols, up, value);
+            }
+            __syncwarp();                                         // before the next row's list comes
+        }
+    }
+}
+template <int J, bool DISTILL>
+__global__ void __launch_bounds__(kRowThreads) short_grad_kernel(VocabGrad p) {
+    grid_release();
+    grid_wait();
+    __shared__ TeacherList lists[DISTILL ? kRowWarps : 1];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    TeacherList& list = lists[DISTILL ? warp : 0];
+    for (size_t row = (size_t)blockIdx.x * kRowWarps + warp; row < p.rows; row += (size_t)gridDim.x * kRowWarps) {
+        const float* x = p.logits + row * p.stride;
+        float* g = p.grad_logits + row * p.stride;
+        if (DISTILL) { list_fetch(list, p, row); copies_end(); }
+        const float m = load_behind(p.row_stats + 2 * row), s = load_behind(p.row_stats + 2 * row + 1);
+        const Terms t = grad_terms<DISTILL>(p, row, m, s);
+        const float x_token = t.token >= 0 ? load_behind(x + t.token) : 0.0f;
+        const ShortRow<J> r(x, p.cols);
+        __syncwarp();                                             // all that is read of the row, before any of it is written (grad_logits may be logits)
+        if (DISTILL) {
+            list_ready(list, p, row);
+            const ProbGrad value = {m, p.c, t.k0};
+            r.write(g, t.none, value);
+            __syncwarp();
+            if (!t.none) list_write(list, p.n_teacher, g, 0, p.cols, t.up, value);
+            __syncwarp();                                         // before the next row's list comes
+        } else {
+            const EntropyGrad value = {m, p.c, t.k0, t.k1};
+            r.write(g, t.none, value);
+            __syncwarp();
+            if (!t.none && lane == 0 && t.token >= 0) g[t.token] = value(x_token) + t.up;
         }
     }
 }
@@ -1196,7 +1346,27 @@ int row_cluster(const VocabRows& p, int sm_count) {
     while (n < kMaxCluster && ((p.rows * 2 * n <= 2 * (size_t)sm_count && p.cols / (2 * n) >= 2048) || (p.rows * 2 * n <= most * sm_count && p.cols / (2 * n) >= least))) n *= 2;
     return n;
 }
+// f(kernel template argument) by the columns
+template <class F>
+cudaError_t short_by_cols(int cols, F f) {
+    return cols <= 512 ? f(std::integral_constant<int, 4>()) : cols <= 1024 ? f(std::integral_constant<int, 8>()) : f(std::integral_constant<int, 16>());
+}
+// Longer ones by warps of 32 quads a lane: 3000 x 4096 statistics 15 / 15 us, their gradient 18 / 23.  Fewer rows than three an SM: 300 x 2000 statistics 3.7 / 3.3 us,
+// their gradient 3.3 / 3.9.
+constexpr int kShortCols = 2048;
+bool short_rows(size_t rows, int cols, int sm_count) { return cols <= kShortCols && rows >= 3 * (size_t)sm_count; }
+unsigned short_grid(size_t rows, int sm_count) {
+    const size_t want = (rows + kRowWarps - 1) / kRowWarps, cap = (size_t)sm_count * 8;
+    return (unsigned)(want < cap ? want : cap);
+}
 cudaError_t launch_forward(VocabRows& p, int sm_count, cudaStream_t stream) {
+    if (p.n_top == 0 && short_rows(p.rows, p.cols, sm_count))
+        return short_by_cols(p.cols, [&](auto j) {
+            constexpr int J = decltype(j)::value;
+            const auto kern = p.n_teacher ? (p.grad_logits ? short_rows_kernel<J, false, kGrad> : short_rows_kernel<J, false, kList>)
+                                          : p.entropy ? short_rows_kernel<J, true, kPlain> : short_rows_kernel<J, false, kPlain>;
+            return launch_rows(kern, short_grid(p.rows, sm_count), kRowThreads, 1, 0, stream, p);
+        });
     p.cluster = row_cluster(p, sm_count);
     // Bounds after 1, 2, 4, 8, ... steps, between two of which there are as many hits again; after 1 and 2 only where a barrier and a bound are more than the
     // hits they save.  All of them / two, k = 20: 4096 x 32000 (8 steps) 112 / 110 us, 2000 x 50003 82 / 86, 600 x 128256 69 / 122; k = 64:
@@ -1264,6 +1434,11 @@ void temperature_of(float t, float* c, float* inv_t) {
     *c = (float)(1.4426950408889634 / (double)t);
 }
 cudaError_t launch_grad(bool distill, VocabGrad& p, int sm_count, cudaStream_t stream) {
+    if (short_rows(p.rows, p.cols, sm_count))
+        return short_by_cols(p.cols, [&](auto j) {
+            constexpr int J = decltype(j)::value;
+            return launch_rows(distill ? short_grad_kernel<J, true> : short_grad_kernel<J, false>, short_grid(p.rows, sm_count), kRowThreads, 1, 0, stream, p);
+        });
     // tiles of a row where the rows are fewer than the CTAs that fill the SMs
     const size_t want = 4 * (size_t)sm_count;
     p.tiles = 1;

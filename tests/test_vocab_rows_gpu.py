@@ -141,6 +141,11 @@ def check_logprobs(ctx, x, stride, k, T, tokens):
     (40, 32000, 64, 0, 64, 0.3),
     (2, 150001, 0, 0, 50, 1.0),
     (300, 32000, 0, 0, 1, 1.0),
+    (500, 500, 0, 0, 0, 1.0),             # a warp a row
+    (3001, 513, 1, 2, 0, 0.5),
+    (1200, 1025, 0, 1, 0, 1.0),
+    (600, 2048, 3, 3, 0, 2.0),
+    (700, 3, 0, 0, 0, 1.0),
     (190, 60003, 1, 0, 20, 1.0),          # two CTAs a row, three on an SM
     (110, 128256, 0, 0, 128, 1.0),
 ])
