@@ -19,7 +19,6 @@
 #include <cfloat>
 #include <climits>
 #include <cmath>
-#include <type_traits>
 
 namespace mcl {
 namespace {
@@ -1184,24 +1183,26 @@ __global__ void __launch_bounds__(kRowThreads, 4) vocab_grad_kernel(VocabGrad p)
     }
 }
 
-// ---- short rows: a warp for each, which holds it in registers ----------------------------------------------------------------
-// Up to 128 J logits, J quads a lane; no barrier, the largest logit is known before the first exponential, and 16 and more rows of an SM are on their way.  What a CTA
-// spends on a row beside its logits, 2.4 us, is more than short rows take: 11000 x 1000 by CTAs / by warps: statistics 47 / 11 us, their gradient 40 / 14, lists' loss
-// 54 / 17, loss and gradient 83 / 27 us; 40000 x 2000: 167 / 54 (92 % of the copy's rate), 161 / 101 (98 %), 177 / 94, 318 / 118 (84 %).
-template <int J>
+// ---- short rows: W warps for each, which hold it in registers ----------------------------------------------------------------
+// Up to 128 W J logits, J quads a lane: a barrier a row at most, no exponential before the warp's largest logit is known, a second look that costs nothing, and as
+// many rows of an SM on their way as registers hold.  What a CTA of the kernel above spends on a row beside its logits, 2.4 us, is more than short rows take.  By such
+// CTAs / here: 11000 x 1000 statistics 47 / 11 us, their gradient 40 / 14, lists' loss 54 / 17, loss and gradient 83 / 27; 40000 x 2000: 167 / 54 (92 % of the copy's rate),
+// 161 / 101 (98 %), 177 / 94, 318 / 118 (84 %); 11000 x 4096 44 / 40, 61 / 59, 63 / 56, 143 / 74.
+template <int W, int J>
 struct ShortRow {
     Part part;
     float4 v[J];
     float loose;                       // outside the quads: one of the first lanes each
     __device__ __forceinline__ ShortRow(const float* row, int n) : part(row, n), loose(-INFINITY) {
-        const int lane = threadIdx.x & 31;
+        const int t = threadIdx.x % (32 * W);
 #pragma unroll
         for (int j = 0; j < J; ++j) {
             v[j] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-            if (lane + 32 * j < part.n4) v[j] = load_behind(part.quads() + lane + 32 * j);
+            if (t + 32 * W * j < part.n4) v[j] = load_behind(part.quads() + t + 32 * W * j);
         }
-        if (lane < part.n - 4 * part.n4) loose = load_behind(part.p + part.loose(lane));
+        if (t < part.n - 4 * part.n4) loose = load_behind(part.p + part.loose(t));
     }
+    // of this warp's part
     template <bool ENTROPY>
     __device__ __forceinline__ Stats<ENTROPY> stats(float c) const {
         float top = fmaxf(-FLT_MAX, loose);
@@ -1221,19 +1222,25 @@ struct ShortRow {
     }
     template <class F>
     __device__ __forceinline__ void write(float* g, bool none, F f) const {
-        const int lane = threadIdx.x & 31;
+        const int t = threadIdx.x % (32 * W);
         const bool vec = ((reinterpret_cast<uintptr_t>(g) ^ reinterpret_cast<uintptr_t>(part.p)) & 15) == 0;
 #pragma unroll
         for (int j = 0; j < J; ++j) {
-            if (lane + 32 * j >= part.n4) continue;
-            float* to = g + part.head + 4 * (lane + 32 * j);
+            if (t + 32 * W * j >= part.n4) continue;
+            float* to = g + part.head + 4 * (t + 32 * W * j);
             const float4 o = none ? make_float4(0.f, 0.f, 0.f, 0.f) : quad_of(v[j], f);
             if (vec) *reinterpret_cast<float4*>(to) = o;
             else { to[0] = o.x; to[1] = o.y; to[2] = o.z; to[3] = o.w; }
         }
-        if (lane < part.n - 4 * part.n4) g[part.loose(lane)] = none ? 0.0f : f(loose);
+        if (t < part.n - 4 * part.n4) g[part.loose(t)] = none ? 0.0f : f(loose);
     }
 };
+// The warps of a row wait for one another.
+template <int W>
+__device__ __forceinline__ void row_sync() {
+    if (W == 1) __syncwarp();
+    else asm volatile("bar.sync %0, %1;" ::"r"(1 + (int)threadIdx.x / (32 * W)), "n"(32 * W) : "memory");
+}
 // A row's list and the logits at its ids (where p has logits to look at), by the warp that has the row.
 template <class P>
 __device__ __forceinline__ void list_ready(TeacherList& l, const P& p, size_t row) {
@@ -1248,77 +1255,87 @@ __device__ __forceinline__ void list_ready(TeacherList& l, const P& p, size_t ro
     copies_wait<0>();
     __syncwarp();
 }
-template <int J, bool ENTROPY, RowWork WORK>
+template <int W, int J, bool ENTROPY, RowWork WORK>
 __global__ void __launch_bounds__(kRowThreads) short_rows_kernel(VocabRows p) {
     constexpr bool DISTILL = WORK == kList || WORK == kGrad, GRAD = WORK == kGrad;
+    constexpr int G = kRowWarps / W;   // rows of a CTA at a time
     grid_release();
     grid_wait();
-    __shared__ TeacherList lists[DISTILL ? kRowWarps : 1];
+    __shared__ TeacherList lists[DISTILL ? G : 1];
+    __shared__ float3 sums[2][kRowWarps];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    TeacherList& list = lists[DISTILL ? warp : 0];
+    const bool lead = warp % W == 0;   // the warp that has the row's list and results
+    TeacherList& list = lists[DISTILL ? warp / W : 0];
     const float up = GRAD ? load_behind(p.grad_out) * p.inv_t / (float)p.rows : 0.0f;
-    for (size_t row = (size_t)blockIdx.x * kRowWarps + warp; row < p.rows; row += (size_t)gridDim.x * kRowWarps) {
+    int turn = 0;
+    for (size_t row = (size_t)blockIdx.x * G + warp / W; row < p.rows; row += (size_t)gridDim.x * G) {
         const float* x = p.logits + row * p.stride;
-        if (DISTILL) { list_fetch(list, p, row); copies_end(); }
+        if (DISTILL && lead) { list_fetch(list, p, row); copies_end(); }
         int token = -1;
         float x_token = 0.0f;
-        if (!DISTILL && p.tokens != nullptr && lane == 0) {
+        if (!DISTILL && p.tokens != nullptr && lead && lane == 0) {
             token = load_behind(p.tokens + row);
             if (token < 0 || token >= p.cols) token = -1;
             else x_token = load_behind(x + token);
         }
-        const ShortRow<J> r(x, p.cols);
-        const Stats<ENTROPY> st = r.template stats<ENTROPY>(p.c);
+        const ShortRow<W, J> r(x, p.cols);
+        Stats<ENTROPY> st = r.template stats<ENTROPY>(p.c);
+        if (DISTILL && lead) list_ready(list, p, row);            // before anything of this row may become its gradient (grad_logits == logits)
+        if (W > 1) {
+            if (lane == 0) sums[turn][warp] = make_float3(st.m, st.s, st.a);
+            row_sync<W>();
+            const float3 part = sums[turn][warp / W * W + (lane & (W - 1))];
+            st.m = part.x; st.s = part.y; st.a = part.z;
+            st.template join<W>(p.c);
+            turn ^= 1;
+        }
         const float m = st.m, s = st.s, log_s = logf(s);
         auto log_prob = [&](float value) { return s == 0.0f ? -INFINITY : (value - m) * p.inv_t - log_s; };      // s == 0: nothing is left of the row
-        if (!DISTILL && lane == 0) {
+        if (!DISTILL && lead && lane == 0) {
             if (p.row_stats != nullptr) { p.row_stats[2 * row] = m; p.row_stats[2 * row + 1] = s; }
             if (p.logprobs != nullptr) p.logprobs[row] = token < 0 ? 0.0f : log_prob(x_token);
             if (ENTROPY) p.entropy[row] = s == 0.0f ? 0.0f : log_s - st.a / s * kLn2;
         }
-        if (DISTILL) {
-            list_ready(list, p, row);
-            list_result(p, list, row, m, s, list_loss(list, p.n_teacher, log_prob));
-            if (GRAD) {
-                const float sg = gradient_sum(s, list.sum);
-                const ProbGrad value = {m, p.c, up / sg};
-                r.write(p.grad_logits + row * p.stride, sg == 0.0f, value);
-                __syncwarp();
-                if (!(sg == 0.0f)) list_write(list, p.n_teacher, p.grad_logits + row * p.stride, 0, p.cols, up, value);
-            }
-            __syncwarp();                                         // before the next row's list comes
+        if (DISTILL && lead) list_result(p, list, row, m, s, list_loss(list, p.n_teacher, log_prob));
+        if (GRAD) {
+            const float sg = gradient_sum(s, list.sum);
+            const ProbGrad value = {m, p.c, up / sg};
+            r.write(p.grad_logits + row * p.stride, sg == 0.0f, value);
+            row_sync<W>();
+            if (lead && !(sg == 0.0f)) list_write(list, p.n_teacher, p.grad_logits + row * p.stride, 0, p.cols, up, value);
         }
+        if (DISTILL) __syncwarp();                                // before the next row's list comes
     }
 }
-template <int J, bool DISTILL>
+template <int W, int J, bool DISTILL>
 __global__ void __launch_bounds__(kRowThreads) short_grad_kernel(VocabGrad p) {
+    constexpr int G = kRowWarps / W;
     grid_release();
     grid_wait();
-    __shared__ TeacherList lists[DISTILL ? kRowWarps : 1];
+    __shared__ TeacherList lists[DISTILL ? G : 1];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    TeacherList& list = lists[DISTILL ? warp : 0];
-    for (size_t row = (size_t)blockIdx.x * kRowWarps + warp; row < p.rows; row += (size_t)gridDim.x * kRowWarps) {
+    const bool lead = warp % W == 0;
+    TeacherList& list = lists[DISTILL ? warp / W : 0];
+    for (size_t row = (size_t)blockIdx.x * G + warp / W; row < p.rows; row += (size_t)gridDim.x * G) {
         const float* x = p.logits + row * p.stride;
         float* g = p.grad_logits + row * p.stride;
-        if (DISTILL) { list_fetch(list, p, row); copies_end(); }
+        if (DISTILL && lead) { list_fetch(list, p, row); copies_end(); }
         const float m = load_behind(p.row_stats + 2 * row), s = load_behind(p.row_stats + 2 * row + 1);
         const Terms t = grad_terms<DISTILL>(p, row, m, s);
-        const float x_token = t.token >= 0 ? load_behind(x + t.token) : 0.0f;
-        const ShortRow<J> r(x, p.cols);
-        __syncwarp();                                             // all that is read of the row, before any of it is written (grad_logits may be logits)
-        if (DISTILL) {
-            list_ready(list, p, row);
-            const ProbGrad value = {m, p.c, t.k0};
-            r.write(g, t.none, value);
-            __syncwarp();
-            if (!t.none) list_write(list, p.n_teacher, g, 0, p.cols, t.up, value);
-            __syncwarp();                                         // before the next row's list comes
-        } else {
-            const EntropyGrad value = {m, p.c, t.k0, t.k1};
-            r.write(g, t.none, value);
-            __syncwarp();
-            if (!t.none && lane == 0 && t.token >= 0) g[t.token] = value(x_token) + t.up;
+        const float x_token = lead && t.token >= 0 ? load_behind(x + t.token) : 0.0f;
+        const ShortRow<W, J> r(x, p.cols);
+        if (DISTILL && lead) list_ready(list, p, row);
+        row_sync<W>();                                            // all that is read of the row, before any of it is written (grad_logits may be logits)
+        const ProbGrad prob = {m, p.c, t.k0};
+        const EntropyGrad with_entropy = {m, p.c, t.k0, t.k1};
+        if (DISTILL) r.write(g, t.none, prob);
+        else r.write(g, t.none, with_entropy);
+        row_sync<W>();
+        if (lead && !t.none) {
+            if (DISTILL) list_write(list, p.n_teacher, g, 0, p.cols, t.up, prob);
+            else if (lane == 0 && t.token >= 0) g[t.token] = with_entropy(x_token) + t.up;
         }
+        if (DISTILL) __syncwarp();                                // before the next row's list comes
     }
 }
 
@@ -1346,26 +1363,32 @@ int row_cluster(const VocabRows& p, int sm_count) {
     while (n < kMaxCluster && ((p.rows * 2 * n <= 2 * (size_t)sm_count && p.cols / (2 * n) >= 2048) || (p.rows * 2 * n <= most * sm_count && p.cols / (2 * n) >= least))) n *= 2;
     return n;
 }
-// f(kernel template argument) by the columns
+// f(warps of a row, quads of a lane) by the columns
+template <int W, int J>
+struct Short { static constexpr int warps = W, quads = J; };
 template <class F>
 cudaError_t short_by_cols(int cols, F f) {
-    return cols <= 512 ? f(std::integral_constant<int, 4>()) : cols <= 1024 ? f(std::integral_constant<int, 8>()) : f(std::integral_constant<int, 16>());
+    if (cols <= 512) return f(Short<1, 4>());
+    if (cols <= 1024) return f(Short<1, 8>());
+    if (cols <= 2048) return f(Short<1, 16>());
+    if (cols <= 4096) return f(Short<2, 16>());
+    return cols <= 8192 ? f(Short<4, 16>()) : f(Short<8, 16>());
 }
-// Longer ones by warps of 32 quads a lane: 3000 x 4096 statistics 15 / 15 us, their gradient 18 / 23.  Fewer rows than three an SM: 300 x 2000 statistics 3.7 / 3.3 us,
-// their gradient 3.3 / 3.9.
-constexpr int kShortCols = 2048;
-bool short_rows(size_t rows, int cols, int sm_count) { return cols <= kShortCols && rows >= 3 * (size_t)sm_count; }
-unsigned short_grid(size_t rows, int sm_count) {
-    const size_t want = (rows + kRowWarps - 1) / kRowWarps, cap = (size_t)sm_count * 8;
+// Up to how many columns.  11000 x 8192 by CTAs / by warps: statistics 60 / 77 us, lists' loss 80 / 82, the gradient of log probabilities 111 / 111, of lists 116 / 111, loss
+// and gradient 225 / 128; 3000 x 16384 of these 77 in the ring / 75.  Fewer rows than three an SM: 300 x 2000 statistics 3.7 / 3.3 us, their gradient 3.3 / 3.9.
+constexpr int kShortStats = 4096, kShortGrad = 4096, kShortListGrad = 8192, kShortBoth = 16384;
+bool short_rows(size_t rows, int cols, int most, int sm_count) { return cols <= most && rows >= 3 * (size_t)sm_count; }
+unsigned short_grid(size_t rows, int warps, int sm_count) {
+    const size_t at_once = kRowWarps / warps, want = (rows + at_once - 1) / at_once, cap = (size_t)sm_count * 8;
     return (unsigned)(want < cap ? want : cap);
 }
 cudaError_t launch_forward(VocabRows& p, int sm_count, cudaStream_t stream) {
-    if (p.n_top == 0 && short_rows(p.rows, p.cols, sm_count))
-        return short_by_cols(p.cols, [&](auto j) {
-            constexpr int J = decltype(j)::value;
-            const auto kern = p.n_teacher ? (p.grad_logits ? short_rows_kernel<J, false, kGrad> : short_rows_kernel<J, false, kList>)
-                                          : p.entropy ? short_rows_kernel<J, true, kPlain> : short_rows_kernel<J, false, kPlain>;
-            return launch_rows(kern, short_grid(p.rows, sm_count), kRowThreads, 1, 0, stream, p);
+    if (p.n_top == 0 && short_rows(p.rows, p.cols, p.grad_logits ? kShortBoth : kShortStats, sm_count))
+        return short_by_cols(p.cols, [&](auto shape) {
+            constexpr int W = decltype(shape)::warps, J = decltype(shape)::quads;
+            const auto kern = p.n_teacher ? (p.grad_logits ? short_rows_kernel<W, J, false, kGrad> : short_rows_kernel<W, J, false, kList>)
+                                          : p.entropy ? short_rows_kernel<W, J, true, kPlain> : short_rows_kernel<W, J, false, kPlain>;
+            return launch_rows(kern, short_grid(p.rows, W, sm_count), kRowThreads, 1, 0, stream, p);
         });
     p.cluster = row_cluster(p, sm_count);
     // Bounds after 1, 2, 4, 8, ... steps, between two of which there are as many hits again; after 1 and 2 only where a barrier and a bound are more than the
@@ -1397,8 +1420,8 @@ Ring ring_of(int cols) {
         }
     return {0, 0, 0};
 }
-// Rows of at least 11264 logits (3000 x 12000 with lists of 64: 86 us, twice out of L2 93; 3000 x 10000: 85 and 77; a row takes the list's warp 4 us however short it
-// is), as many as keep all SMs busy, gradients on the logits' 16-byte boundaries.
+// Rows of at least 11264 logits (300 x 12000 with lists of 64: 16.2 us, twice out of L2 16.4; 3000 x 10000: 85 and 77; a row takes the list's warp 4 us however short
+// it is) that are not for short_rows_kernel, as many as keep all SMs busy, gradients on the logits' 16-byte boundaries.
 // Longer ones by as many CTAs as hold a row: more of them are more clusters' seams and fewer clusters that fit the GPU (1000 x 128256 by 3 / 4 / 6: 222 / 240 / 252 us,
 // 400 x 262144 by 6 / 8: 193 / 223, 2000 x 60000 by 2 / 3: 190 / 223; twice out of L2 298, 256 and 285).
 bool ring_takes(VocabRows& p, int sm_count, size_t max_smem) {
@@ -1407,7 +1430,7 @@ bool ring_takes(VocabRows& p, int sm_count, size_t max_smem) {
         if (p.cluster == kMaxCluster) return false;
     // few rows: in parts of no fewer than 11264 (200 x 32000 by one CTA 25 us, by two, twice out of L2, 21.6, by two here 18.2)
     while (p.rows * p.cluster < 2 * (size_t)sm_count && p.cluster < kMaxCluster && p.cols / (p.cluster + 1) >= 11264) ++p.cluster;
-    return p.cols >= 11264 && p.rows * p.cluster >= 2 * (size_t)sm_count && kRingBytes + kRingLists * sizeof(TeacherList) + 2048 <= max_smem &&
+    return p.cols >= 11264 && !short_rows(p.rows, p.cols, kShortBoth, sm_count) && p.rows * p.cluster >= 2 * (size_t)sm_count && kRingBytes + kRingLists * sizeof(TeacherList) + 2048 <= max_smem &&
            ((reinterpret_cast<uintptr_t>(p.logits) ^ reinterpret_cast<uintptr_t>(p.grad_logits)) & 15) == 0;
 }
 cudaError_t launch_ring(VocabRows& p, int sm_count, cudaStream_t stream) {
@@ -1434,10 +1457,10 @@ void temperature_of(float t, float* c, float* inv_t) {
     *c = (float)(1.4426950408889634 / (double)t);
 }
 cudaError_t launch_grad(bool distill, VocabGrad& p, int sm_count, cudaStream_t stream) {
-    if (short_rows(p.rows, p.cols, sm_count))
-        return short_by_cols(p.cols, [&](auto j) {
-            constexpr int J = decltype(j)::value;
-            return launch_rows(distill ? short_grad_kernel<J, true> : short_grad_kernel<J, false>, short_grid(p.rows, sm_count), kRowThreads, 1, 0, stream, p);
+    if (short_rows(p.rows, p.cols, distill ? kShortListGrad : kShortGrad, sm_count))
+        return short_by_cols(p.cols, [&](auto shape) {
+            constexpr int W = decltype(shape)::warps, J = decltype(shape)::quads;
+            return launch_rows(distill ? short_grad_kernel<W, J, true> : short_grad_kernel<W, J, false>, short_grid(p.rows, W, sm_count), kRowThreads, 1, 0, stream, p);
         });
     // tiles of a row where the rows are fewer than the CTAs that fill the SMs
     const size_t want = 4 * (size_t)sm_count;

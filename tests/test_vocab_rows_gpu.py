@@ -146,6 +146,9 @@ def check_logprobs(ctx, x, stride, k, T, tokens):
     (1200, 1025, 0, 1, 0, 1.0),
     (600, 2048, 3, 3, 0, 2.0),
     (700, 3, 0, 0, 0, 1.0),
+    (500, 2049, 1, 1, 0, 1.0),            # two warps
+    (450, 4096, 0, 0, 0, 0.7),
+    (450, 8189, 1, 3, 0, 1.0),            # four
     (190, 60003, 1, 0, 20, 1.0),          # two CTAs a row, three on an SM
     (110, 128256, 0, 0, 128, 1.0),
 ])
@@ -179,6 +182,23 @@ def test_top_tokens_of_rows_of_many_steps(ctx, R, V, k, rounded):
     tokens = torch.full((R,), 0)
     tokens[5], tokens[6], tokens[7] = V - 1, V // 2, 1
     check_logprobs(ctx, x, stride, k, 1.0, tokens)
+
+
+@pytest.mark.parametrize("R,V", [(460, 5), (450, 511), (500, 1500), (447, 3999), (447, 8001)])
+def test_short_rows_that_go_wrong(ctx, R, V):
+    x, stride = make_logits(R, V, 1, 1, seed=7)
+    special_rows(x)
+    tokens = torch.full((R,), 0)
+    tokens[5], tokens[6], tokens[7], tokens[8], tokens[9] = V - 1, V // 2, 1, -1, V
+    check_logprobs(ctx, x, stride, 0, 1.0, tokens)
+    x[10, V // 3] = math.nan
+    x[11, V - 1] = math.inf
+    x[12] = math.nan
+    got = run_logprobs(ctx, x, stride, tokens.to("cuda", torch.int32), 0, 1.0)
+    bad = torch.zeros(R, dtype=torch.bool)
+    bad[10:13] = True
+    for n in ("logp", "H"):
+        assert torch.equal(torch.isnan(got[n]).cpu(), bad), n
 
 
 def test_top_tokens_where_one_thread_has_all_large_values(ctx):
@@ -261,7 +281,7 @@ def policy_grad(want, tokens, dlogp, dent):
 
 
 @pytest.mark.parametrize("R,V,pad,offset,T", [(1, 1, 0, 0, 1.0), (9, 130, 1, 1, 0.5), (70, 1001, 0, 2, 1.0), (8, 32000, 0, 0, 2.0), (1, 50003, 2, 1, 1.0),
-                                             (700, 2048, 0, 0, 1.0), (2600, 515, 0, 0, 0.7)])
+                                             (700, 2048, 0, 0, 1.0), (2600, 515, 0, 0, 0.7), (460, 4001, 1, 1, 1.0), (450, 8192, 0, 0, 2.0)])
 @pytest.mark.parametrize("which", ["both", "logp", "entropy"])
 @pytest.mark.parametrize("in_place", [False, True])
 def test_token_logprobs_backward(ctx, R, V, pad, offset, T, which, in_place):
@@ -418,6 +438,8 @@ FORMS = ["one call", "split", "in place", "split in place"]
 
 @pytest.mark.parametrize("R,V,K,pad,offset,T", [(1, 1, 1, 0, 0, 1.0), (3, 5, 5, 1, 1, 2.0), (20, 128, 128, 0, 0, 1.0), (33, 1001, 7, 0, 2, 0.5), (600, 2500, 64, 0, 0, 2.0),
                                               (2500, 300, 3, 1, 0, 1.0), (1, 32000, 20, 0, 0, 1.0), (12, 33001, 128, 3, 1, 1.5), (40, 32000, 64, 0, 0, 4.0),
+                                              (900, 1000, 128, 0, 1, 1.0), (455, 2047, 33, 2, 3, 0.5), (1000, 4001, 64, 1, 0, 2.0), (600, 8190, 20, 0, 0, 1.0),
+                                              (450, 9001, 64, 1, 0, 1.0), (446, 16384, 8, 0, 0, 1.0),
                                               (300, 24581, 5, 0, 0, 1.0), (450, 32000, 64, 0, 0, 2.0), (310, 33001, 33, 3, 1, 0.7), (297, 45056, 128, 4, 3, 1.0)])
 @pytest.mark.parametrize("form", FORMS)
 def test_distillation(ctx, R, V, K, pad, offset, T, form):
@@ -459,7 +481,7 @@ def test_distillation_of_long_rows(ctx, R, V, K, pad, offset, T, form):
 
 
 @pytest.mark.parametrize("form", FORMS)
-@pytest.mark.parametrize("R,V", [(16, 500), (16, 40000), (320, 26000)])
+@pytest.mark.parametrize("R,V", [(16, 500), (16, 40000), (320, 26000), (460, 500), (460, 1500), (460, 3001), (450, 7777)])
 def test_distillation_lists_and_rows_that_go_wrong(ctx, R, V, form):
     K = 10
     x, stride = make_logits(R, V, 1, 0, seed=11)
@@ -509,7 +531,7 @@ def test_distillation_lists_longer_than_a_warp(ctx, K, form):
 
 
 @pytest.mark.parametrize("form", ["one call", "split"])
-@pytest.mark.parametrize("R,V", [(7, 3000), (300, 25001), (160, 60001)])
+@pytest.mark.parametrize("R,V", [(7, 3000), (300, 25001), (160, 60001), (460, 900), (460, 2500), (450, 8000)])
 def test_distillation_of_rows_with_nan(ctx, R, V, form):
     K = 5
     x, stride = make_logits(R, V, seed=12)
