@@ -343,8 +343,8 @@ int mcl_cuda_gqa_backward(mcl_cuda_ctx* ctx, const float* q, const float* k, con
  *                        NULL; out may be x; row_stats [rows, 2] receives the mean and 1 / sqrt(var + eps) (NULL: not kept)
  *   layernorm_backward   from the row_stats of the forward call: grad_x [rows, cols], grad_weight and grad_bias [cols] (overwritten, not
  *                        added to); any of the three may be NULL.  grad_x may be grad_out or x itself.  Sums over the rows have a fixed
- *                        order: the same call gives the same bits.  Takes workspace for partial sums, at most 8 MiB up to 4096 columns.
- * ---- */
+ *                        order: the same call gives the same bits.  Takes workspace for partial sums, up to 8192 columns 10 MB at most.
+ * cols is 2^30 at most. ---- */
 int mcl_cuda_layernorm(mcl_cuda_ctx* ctx, const float* x, const float* weight, const float* bias, float* out, float* row_stats, size_t rows,
                        size_t cols, float eps);
 int mcl_cuda_layernorm_backward(mcl_cuda_ctx* ctx, const float* x, const float* weight, const float* grad_out, const float* row_stats,
@@ -352,7 +352,7 @@ int mcl_cuda_layernorm_backward(mcl_cuda_ctx* ctx, const float* x, const float* 
 
 /* ---- what rows of logits say about tokens, and what they learn from a teacher's (no reference counterpart; next to softmax_cross_entropy
  * above).  logits [rows, cols] with row_stride >= cols floats from row to row; columns behind cols are neither read nor written.  p = the
- * softmax of a row's logits / temperature.
+ * softmax of a row's logits / temperature (1e-30 to 1e30).  cols is 2^30 at most.  No workspace; the same call gives the same bits.
  *   token_logprobs            logprobs [rows] = ln p of the row's token (0 for a token outside [0, cols): padding; tokens and logprobs may be
  *                             NULL together); entropy [rows] (or NULL) = -sum p ln p; top_ids, top_logprobs [rows, n_top] (one of them may be
  *                             NULL, both with n_top = 0): the n_top largest logits' places and ln p, largest first, equal ones by their
@@ -366,8 +366,9 @@ int mcl_cuda_layernorm_backward(mcl_cuda_ctx* ctx, const float* x, const float* 
  *                             outside [0, cols) is no entry, a row without entries has loss 0; an id named twice is two entries.  With
  *                             grad_out and grad_logits (both or neither) also grad_logits = grad_out[0] * the gradient of out[0], in the same
  *                             pass over the logits.  No factor temperature^2 is applied.
- *   ..._backward              the same gradient from row_stats, for a grad_out that is known later
- * grad_logits has the logits' stride, may be the logits themselves, and is exactly 0 in rows that nothing asks anything of (a token or ids
+ *   ..._backward              the same gradient from row_stats, for a grad_out that is known later.  These row_stats are distillation_loss's own: s is 0
+ *                             in a row without entries, and not a number where the list is none
+ * grad_logits has the logits' stride, may be the logits themselves but overlap them in no other way, and is exactly 0 in rows that nothing asks anything of (a token or ids
  * outside the vocabulary and no other gradient, or gradients of 0), whatever these rows hold.
  * Logits of -infinity (or the lowest float) are masked: p = 0, no part in the entropy, gradient 0.  A row of nothing but -infinity has
  * logprobs and top_logprobs -infinity, entropy 0, an infinite distillation loss (0 without entries) and gradient 0.  A row with a NaN or +infinity gives NaN, and ids

@@ -1358,7 +1358,7 @@ cudaError_t launch_rows(void (*kern)(P...), unsigned grid, int threads, int clus
 // parts on: 150 x 24000 19 / 17.6, 200 x 14000 14.4 / 12.8.
 int row_cluster(const VocabRows& p, int sm_count) {
     const size_t most = p.n_top ? 3 : 4;
-    const int least = p.grad_logits ? 6144 : p.n_top || p.n_teacher ? 24576 : 30720;
+    const int least = p.grad_logits ? 6144 : p.n_top || p.n_teacher ? 24576 : 30000;
     int n = 1;
     while (n < kMaxCluster && ((p.rows * 2 * n <= 2 * (size_t)sm_count && p.cols / (2 * n) >= 2048) || (p.rows * 2 * n <= most * sm_count && p.cols / (2 * n) >= least))) n *= 2;
     return n;
