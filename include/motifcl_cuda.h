@@ -352,7 +352,8 @@ int mcl_cuda_layernorm_backward(mcl_cuda_ctx* ctx, const float* x, const float* 
 
 /* ---- what rows of logits say about tokens, and what they learn from a teacher's (no reference counterpart; next to softmax_cross_entropy
  * above).  logits [rows, cols] with row_stride >= cols floats from row to row; columns behind cols are neither read nor written.  p = the
- * softmax of a row's logits / temperature (1e-30 to 1e30).  cols is 2^30 at most.  No workspace; the same call gives the same bits.
+ * softmax of a row's logits / temperature (1e-30 to 1e30).  cols is 2^30 at most.  No workspace.  The same call gives the same bits; one that
+ * asks for other outputs, or has other alignment, may round differently.
  *   token_logprobs            logprobs [rows] = ln p of the row's token (0 for a token outside [0, cols): padding; tokens and logprobs may be
  *                             NULL together); entropy [rows] (or NULL) = -sum p ln p; top_ids, top_logprobs [rows, n_top] (one of them may be
  *                             NULL, both with n_top = 0): the n_top largest logits' places and ln p, largest first, equal ones by their

@@ -1235,6 +1235,105 @@ struct ShortRow {
         if (t < part.n - 4 * part.n4) g[part.loose(t)] = none ? 0.0f : f(loose);
     }
 };
+// The k largest of a row that a warp has, k <= kMaxList and the row's length: f(rank, candidate).  A bound that at least k values reach: the k-th largest of the largest of
+// four groups of every lane, found by halving; those that reach it go to `list`, kCandidates places, and are ordered by counting.
+template <int J, class F>
+__device__ __forceinline__ void short_tops(const ShortRow<1, J>& r, int k, unsigned long long* list, F f) {
+    const int lane = threadIdx.x & 31, n4 = r.part.n4;
+    const bool has_loose = lane < r.part.n - 4 * n4;
+    // the largest t of [lo, hi) with count(t) >= k, or one with k <= count(t) <= most; count(lo) >= k > count(hi)
+    auto halve = [&](uint32_t& lo, uint32_t hi, int most, auto count) {
+        while (hi - lo > 1) {
+            const uint32_t mid = lo + (hi - lo) / 2;
+            const int n = (int)__reduce_add_sync(0xffffffffu, (unsigned)count(unordered(mid)));
+            if (n < k) hi = mid;
+            else {
+                lo = mid;
+                if (n <= most) return;
+            }
+        }
+    };
+    float top[4];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        top[g] = g == 0 ? r.loose : -INFINITY;
+#pragma unroll
+        for (int j = g; j < J; j += 4) top[g] = fmaxf(top[g], top_of(r.v[j]));
+    }
+    const uint32_t all = ordered(-INFINITY), high = __reduce_max_sync(0xffffffffu, ordered(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]))));
+    uint32_t bound = k == 1 ? high : all;
+    if (k > 1) halve(bound, high + 1, k, [&](float t) { return (top[0] >= t) + (top[1] >= t) + (top[2] >= t) + (top[3] >= t); });
+    auto reach = [&](float t) {                                   // how many of the lane's
+        int n = has_loose && r.loose >= t;
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+            if (lane + 32 * j < n4) n += (r.v[j].x >= t) + (r.v[j].y >= t) + (r.v[j].z >= t) + (r.v[j].w >= t);
+        return n;
+    };
+    float least = unordered(bound);
+    int mine = reach(least), n = (int)__reduce_add_sync(0xffffffffu, (unsigned)mine);
+    bool fill = false;
+    if (n > max(k + 32, 96)) {                                    // counting takes n^2 steps, halving 10 to 32 looks at the row
+        halve(bound, high + 1, k + 32, reach);
+        least = unordered(bound);
+        mine = reach(least);
+        n = (int)__reduce_add_sync(0xffffffffu, (unsigned)mine);
+        fill = n > kCandidates;                                   // that many are equal to it, and fewer than k above
+    }
+    // those that pass, to where the lanes in front of this one end
+    auto put = [&](auto pass, int to) {
+        auto one = [&](float v, int at) { if (pass(v)) { if (to < kCandidates) list[to] = candidate(v, at); ++to; } };
+        if (has_loose) one(r.loose, r.part.loose(lane));
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            const int at = r.part.head + 4 * (lane + 32 * j);
+            if (lane + 32 * j < n4 && pass(top_of(r.v[j]))) { one(r.v[j].x, at); one(r.v[j].y, at + 1); one(r.v[j].z, at + 2); one(r.v[j].w, at + 3); }
+        }
+    };
+    auto in_front = [&](int v) {                                  // of the lanes in front of this one
+        int sum = v;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int other = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += other;
+        }
+        return sum - v;
+    };
+    if (!fill) put([&](float v) { return v >= least; }, in_front(mine));
+    else {
+        const float above = unordered(bound + 1);                 // the next float: v >= above is v > least
+        mine = reach(above);
+        put([&](float v) { return v >= above; }, in_front(mine));
+        n = (int)__reduce_add_sync(0xffffffffu, (unsigned)mine);
+        // the first of those equal to it: in front of the quads, in them, behind them
+        auto some = [&](bool a, bool b, bool c, bool d, int at) {
+            const int m = a + b + c + d;
+            int to = n + in_front(m);
+            if (a) { if (to < k) list[to] = candidate(least, at); ++to; }
+            if (b) { if (to < k) list[to] = candidate(least, at + 1); ++to; }
+            if (c) { if (to < k) list[to] = candidate(least, at + 2); ++to; }
+            if (d && to < k) list[to] = candidate(least, at + 3);
+            n = min(k, n + (int)__reduce_add_sync(0xffffffffu, (unsigned)m));
+        };
+        some(lane < r.part.head && r.loose == least, false, false, false, lane);
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            const bool in = lane + 32 * j < n4;
+            some(in && r.v[j].x == least, in && r.v[j].y == least, in && r.v[j].z == least, in && r.v[j].w == least, r.part.head + 4 * (lane + 32 * j));
+        }
+        some(lane >= r.part.head && has_loose && r.loose == least, false, false, false, r.part.loose(lane));
+    }
+    __syncwarp();
+#pragma unroll 1
+    for (int i = lane; i < n; i += 32) {
+        const unsigned long long v = list[i];
+        int rank = 0;
+#pragma unroll 4
+        for (int j = 0; j < n; ++j) rank += list[j] > v;
+        if (rank < k) f(rank, v);
+    }
+    __syncwarp();                                                 // before the next row's candidates come
+}
 // The warps of a row wait for one another.
 template <int W>
 __device__ __forceinline__ void row_sync() {
@@ -1257,12 +1356,14 @@ __device__ __forceinline__ void list_ready(TeacherList& l, const P& p, size_t ro
 }
 template <int W, int J, bool ENTROPY, RowWork WORK>
 __global__ void __launch_bounds__(kRowThreads) short_rows_kernel(VocabRows p) {
-    constexpr bool DISTILL = WORK == kList || WORK == kGrad, GRAD = WORK == kGrad;
+    constexpr bool DISTILL = WORK == kList || WORK == kGrad, GRAD = WORK == kGrad, TOP = WORK == kTop;
     constexpr int G = kRowWarps / W;   // rows of a CTA at a time
+    static_assert(!TOP || W == 1, "a warp seeks the largest of its row");
     grid_release();
     grid_wait();
     __shared__ TeacherList lists[DISTILL ? G : 1];
     __shared__ float3 sums[2][kRowWarps];
+    __shared__ unsigned long long candidates[TOP ? kRowWarps : 1][kCandidates];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const bool lead = warp % W == 0;   // the warp that has the row's list and results
     TeacherList& list = lists[DISTILL ? warp / W : 0];
@@ -1295,6 +1396,15 @@ __global__ void __launch_bounds__(kRowThreads) short_rows_kernel(VocabRows p) {
             if (p.row_stats != nullptr) { p.row_stats[2 * row] = m; p.row_stats[2 * row + 1] = s; }
             if (p.logprobs != nullptr) p.logprobs[row] = token < 0 ? 0.0f : log_prob(x_token);
             if (ENTROPY) p.entropy[row] = s == 0.0f ? 0.0f : log_s - st.a / s * kLn2;
+        }
+        if constexpr (TOP) {
+            const size_t at = row * (size_t)p.n_top;
+            auto put = [&](int rank, int id, float value) {
+                if (p.top_ids != nullptr) p.top_ids[at + rank] = id;
+                if (p.top_logprobs != nullptr) p.top_logprobs[at + rank] = value;
+            };
+            if (s == s) short_tops(r, p.n_top, candidates[warp], [&](int rank, unsigned long long c) { put(rank, (int)(0xffffffffu - (uint32_t)c), log_prob(unordered((uint32_t)(c >> 32)))); });
+            else for (int i = lane; i < p.n_top; i += 32) put(i, -1, s);       // not a number
         }
         if (DISTILL && lead) list_result(p, list, row, m, s, list_loss(list, p.n_teacher, log_prob));
         if (GRAD) {
@@ -1376,16 +1486,26 @@ cudaError_t short_by_cols(int cols, F f) {
 }
 // Up to how many columns.  11000 x 8192 by CTAs / by warps: statistics 60 / 77 us, lists' loss 80 / 82, the gradient of log probabilities 111 / 111, of lists 116 / 111, loss
 // and gradient 225 / 128; 3000 x 16384 of these 77 in the ring / 75.  Fewer rows than three an SM: 300 x 2000 statistics 3.7 / 3.3 us, their gradient 3.3 / 3.9.
-constexpr int kShortStats = 4096, kShortGrad = 4096, kShortListGrad = 8192, kShortBoth = 16384;
+// With tokens sought: 600 x 2000 with 20 / 64 of them 9.1 / 9.0 us and 13 / 17 (four rows an SM), 11000 x 2000 99 / 46 and 143 / 81, 3000 x 1000 28 / 10 and 41 / 16.  Below 1024
+// columns a CTA has warps without values, which leave it no bound: 1 x 500 18 / 5.5 us, 11000 x 500 769 / 19; 1 x 1024 4.5 / 6.3.  Statistics alone, which are
+// the same bits then: 20 x 1000 2.6 / 2.6.
+constexpr int kShortAll = 1023, kShortTop = 2048, kShortStats = 4096, kShortGrad = 4096, kShortListGrad = 8192, kShortBoth = 16384;
 bool short_rows(size_t rows, int cols, int most, int sm_count) { return cols <= most && rows >= 3 * (size_t)sm_count; }
+bool short_forward(const VocabRows& p, int sm_count) {
+    if (p.n_teacher == 0 && p.cols <= kShortAll) return true;
+    if (p.n_top) return short_rows(p.rows / 2, p.cols, kShortTop, sm_count);
+    return short_rows(p.rows, p.cols, p.grad_logits ? kShortBoth : kShortStats, sm_count);
+}
 unsigned short_grid(size_t rows, int warps, int sm_count) {
     const size_t at_once = kRowWarps / warps, want = (rows + at_once - 1) / at_once, cap = (size_t)sm_count * 8;
     return (unsigned)(want < cap ? want : cap);
 }
 cudaError_t launch_forward(VocabRows& p, int sm_count, cudaStream_t stream) {
-    if (p.n_top == 0 && short_rows(p.rows, p.cols, p.grad_logits ? kShortBoth : kShortStats, sm_count))
+    if (short_forward(p, sm_count))
         return short_by_cols(p.cols, [&](auto shape) {
             constexpr int W = decltype(shape)::warps, J = decltype(shape)::quads;
+            if constexpr (W == 1)
+                if (p.n_top) return launch_rows(p.entropy ? short_rows_kernel<W, J, true, kTop> : short_rows_kernel<W, J, false, kTop>, short_grid(p.rows, W, sm_count), kRowThreads, 1, 0, stream, p);
             const auto kern = p.n_teacher ? (p.grad_logits ? short_rows_kernel<W, J, false, kGrad> : short_rows_kernel<W, J, false, kList>)
                                           : p.entropy ? short_rows_kernel<W, J, true, kPlain> : short_rows_kernel<W, J, false, kPlain>;
             return launch_rows(kern, short_grid(p.rows, W, sm_count), kRowThreads, 1, 0, stream, p);

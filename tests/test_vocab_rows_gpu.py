@@ -201,6 +201,34 @@ def test_short_rows_that_go_wrong(ctx, R, V):
         assert torch.equal(torch.isnan(got[n]).cpu(), bad), n
 
 
+@pytest.mark.parametrize("R,V,k,pad,offset", [(460, 5, 5, 0, 0), (447, 100, 100, 1, 1), (450, 511, 20, 1, 0), (500, 512, 128, 0, 0), (450, 700, 64, 3, 2), (890, 1024, 1, 0, 0),
+                                              (900, 1025, 127, 0, 3), (1000, 2047, 2, 1, 1), (900, 2048, 128, 0, 0), (888, 2045, 20, 0, 1),
+                                              (30, 900, 50, 0, 1), (21, 1023, 128, 1, 0)])
+@pytest.mark.parametrize("rounded", [False, True])
+def test_top_tokens_of_short_rows(ctx, R, V, k, pad, offset, rounded):
+    x, stride = make_logits(R, V, pad, offset, seed=8, rounded=rounded)
+    special_rows(x)
+    g = torch.Generator().manual_seed(V + k)
+    x[8] = (torch.arange(V) % 3 == 0).float().to(x.device)               # two values: more equal ones than are collected
+    x[9] = torch.where(torch.arange(V) % 2 == 0, 0.0, -0.0).to(x.device)  # zeros of both signs are equal
+    x[10] = torch.randint(0, 7, (V,), generator=g).float().to(x.device)
+    x[11] = torch.where(torch.rand(V, generator=g) < 0.97, NEG, 1.0).to(x.device)
+    x[12] = torch.where(torch.rand(V, generator=g) < 0.5, -1e-45, 1e-45).to(x.device)
+    x[13] = torch.arange(V, 0, -1, device=x.device) * 1e-3
+    x[14, ::32] += 40.0
+    x[15, : V // 2] += 40.0
+    x[16, 0], x[17, V - 1] = 99.0, 99.0
+    tokens = torch.randint(0, V, (R,), generator=g)
+    check_logprobs(ctx, x, stride, k, 1.0, tokens)
+    x[18, V // 3], x[19, V // 2], x[20] = math.nan, math.inf, math.nan
+    got = run_logprobs(ctx, x, stride, tokens.to("cuda", torch.int32), k, 1.0)
+    assert bool((got["ids"][18:21] == -1).all()) and bool(torch.isnan(got["top"][18:21]).all())
+    ids = top_of(x, k)
+    ok = torch.ones(R, dtype=torch.bool)
+    ok[18:21] = False
+    assert torch.equal(got["ids"].cpu().long()[ok], ids[ok])
+
+
 def test_top_tokens_where_one_thread_has_all_large_values(ctx):
     """More values above a bound from the threads' largest than are collected at once."""
     V, k = 32000, 128
