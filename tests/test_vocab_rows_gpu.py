@@ -658,6 +658,48 @@ def test_two_contexts_at_once(ctx):
     other.close()
 
 
+@pytest.mark.parametrize("R,V", [(300, 30000), (160, 60001), (460, 700), (460, 9001)])
+def test_distillation_recorded_and_on_two_contexts_at_once(ctx, R, V):
+    """Rings of chunks, clusters of them, and warps a row: the same bits alone, replayed with new inputs, and while another context runs the same."""
+    from motifcl_b200 import Context
+    K = 12
+    x, y = make_logits(R, V, seed=32)[0], make_logits(R, V, seed=33)[0]
+    ids, a = (t.to("cuda") for t in make_teacher(R, V, K, 8))
+    one = torch.ones(1, device="cuda")
+    outs = lambda: (torch.empty(R, device="cuda"), torch.empty(1, device="cuda"), torch.empty(R, 2, device="cuda"), torch.empty(R, V, device="cuda"))
+
+    def step(c, t, o):
+        c.distillation_loss(t, ids, a, o[0], o[1], o[2], one, o[3], R, V, K)
+
+    same = lambda p, q: all(torch.equal(u.view(torch.int32), v.view(torch.int32)) for u, v in zip(p, q))
+    want, got = [outs(), outs()], [outs(), outs()]
+    other = Context(0)
+    torch.cuda.synchronize()
+    step(ctx, x, want[0])
+    step(ctx, y, want[1])
+    ctx.finish()
+    for _ in range(4):
+        step(ctx, x, got[0])
+        step(other, y, got[1])
+    ctx.finish()
+    other.finish()
+    assert same(want[0], got[0]) and same(want[1], got[1])
+    ctx.batch_begin()
+    step(ctx, x, got[0])
+    batch = ctx.batch_end()
+    x.copy_(y)
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for t in got[0]:
+            t.zero_()
+        torch.cuda.synchronize()
+        batch.launch()
+        ctx.finish()
+        assert same(want[1], got[0])
+    batch.close()
+    other.close()
+
+
 def test_a_row_beyond_32_bits_of_offset(ctx):
     """2.2e9 floats from the first row to the last: 8.9 GB, of which three rows are looked at."""
     V, stride = 1000, 50_000_000
