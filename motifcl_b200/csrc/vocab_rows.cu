@@ -1417,6 +1417,65 @@ __global__ void __launch_bounds__(kRowThreads) short_rows_kernel(VocabRows p) {
         if (DISTILL) __syncwarp();                                // before the next row's list comes
     }
 }
+// The most probable tokens of a row that a CTA holds: one bound, of all the row, and what reaches it straight out of the registers.
+template <int J, bool ENTROPY>
+__global__ void __launch_bounds__(kRowThreads, 2) held_tops_kernel(VocabRows p) {
+    grid_release();
+    grid_wait();
+    __shared__ Selection z;
+    __shared__ float3 sums[2][kRowWarps];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, k = p.n_top;
+    if (threadIdx.x == 0) z.n_list[0] = z.n_list[1] = 0;
+    int turn = 0;
+    for (size_t row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
+        const float* x = p.logits + row * p.stride;
+        int token = -1;
+        float x_token = 0.0f;
+        if (p.tokens != nullptr && threadIdx.x == kResultThread) {
+            token = load_behind(p.tokens + row);
+            if (token < 0 || token >= p.cols) token = -1;
+            else x_token = load_behind(x + token);
+        }
+        const ShortRow<kRowWarps, J> r(x, p.cols);
+        Stats<ENTROPY> st = r.template stats<ENTROPY>(p.c);
+        if (lane == 0) sums[turn][warp] = make_float3(st.m, st.s, st.a);
+        float top = r.loose;
+#pragma unroll
+        for (int j = 0; j < J; ++j) top = fmaxf(top, top_of(r.v[j]));
+        const float least = unordered(max(bound_of(ordered(top), k, z.bound[turn]), ordered(-INFINITY)));      // a barrier in there: the sums are there too
+        int* count = &z.n_list[turn];
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            const int i = threadIdx.x + kRowThreads * j;
+            if (i < r.part.n4 && top_of(r.v[j]) >= least) take(z, count, r.v[j], r.part.head + 4 * i, least, false);
+        }
+        if ((int)threadIdx.x < r.part.n - 4 * r.part.n4) take(z, count, alone(r.loose), r.part.loose(threadIdx.x), least, false);
+        const float3 part = sums[turn][lane & (kRowWarps - 1)];
+        st.m = part.x; st.s = part.y; st.a = part.z;
+        st.template join<kRowWarps>(p.c);
+        const float m = st.m, s = st.s, log_s = logf(s);
+        auto log_prob = [&](float value) { return s == 0.0f ? -INFINITY : (value - m) * p.inv_t - log_s; };      // s == 0: nothing is left of the row
+        if (threadIdx.x == kResultThread) {
+            if (p.row_stats != nullptr) { p.row_stats[2 * row] = m; p.row_stats[2 * row + 1] = s; }
+            if (p.logprobs != nullptr) p.logprobs[row] = token < 0 ? 0.0f : log_prob(x_token);
+            if (ENTROPY) p.entropy[row] = s == 0.0f ? 0.0f : log_s - st.a / s * kLn2;
+        }
+        __syncthreads();
+        int n = *count;
+        if (threadIdx.x == 0) z.n_list[turn ^ 1] = 0;             // for the next row
+        const size_t at = row * (size_t)k;
+        auto put = [&](int rank, int id, float value) {
+            if (p.top_ids != nullptr) p.top_ids[at + rank] = id;
+            if (p.top_logprobs != nullptr) p.top_logprobs[at + rank] = value;
+        };
+        if (!(s == s)) {                                          // not a number: its places are not looked at
+            if ((int)threadIdx.x < k) put(threadIdx.x, -1, s);
+            continue;
+        }
+        if (n > kCandidates) n = take_few(z, count, r.part.p, r.part.n, 0, least, k, k);
+        each_best(z.list, n, k, [&](int rank, unsigned long long c) { put(rank, (int)(0xffffffffu - (uint32_t)c), log_prob(unordered((uint32_t)(c >> 32)))); });
+    }
+}
 template <int W, int J, bool DISTILL>
 __global__ void __launch_bounds__(kRowThreads) short_grad_kernel(VocabGrad p) {
     constexpr int G = kRowWarps / W;
@@ -1500,7 +1559,21 @@ unsigned short_grid(size_t rows, int warps, int sm_count) {
     const size_t at_once = kRowWarps / warps, want = (rows + at_once - 1) / at_once, cap = (size_t)sm_count * 8;
     return (unsigned)(want < cap ? want : cap);
 }
+// Where rows are few, and no longer than a CTA holds: half the chain of a row (no bounds and notes on the way, no cluster).  Through vocab_rows_kernel / here, 20 tokens:
+// 1 x 8000 6.5 / 4.5 us, 30 x 16384 7.8 / 6.5, 148 x 12345 10.1 / 6.5, 777 x 12345 21 / 19, 600 x 2000 9.1 / 9.6, 1184 x 12345 24.9 / 24.9, 4096 x 8000 56 / 59: a row takes
+// registers that two or three CTAs an SM have, and no copies ahead.
+bool held_tops(const VocabRows& p, int sm_count) {
+    return p.n_top > 0 && p.cols > kShortAll && p.cols <= 64 * kRowThreads && p.rows <= (p.cols >= 4096 ? 6 : 3) * (size_t)sm_count;
+}
+cudaError_t launch_held_tops(const VocabRows& p, int sm_count, cudaStream_t stream) {
+    const size_t cap = (size_t)sm_count * 4;
+    const auto kern = p.cols <= 16 * kRowThreads ? (p.entropy ? held_tops_kernel<4, true> : held_tops_kernel<4, false>)
+                    : p.cols <= 32 * kRowThreads ? (p.entropy ? held_tops_kernel<8, true> : held_tops_kernel<8, false>)
+                                                 : (p.entropy ? held_tops_kernel<16, true> : held_tops_kernel<16, false>);
+    return launch_rows(kern, (unsigned)(p.rows < cap ? p.rows : cap), kRowThreads, 1, 0, stream, p);
+}
 cudaError_t launch_forward(VocabRows& p, int sm_count, cudaStream_t stream) {
+    if (held_tops(p, sm_count)) return launch_held_tops(p, sm_count, stream);
     if (short_forward(p, sm_count))
         return short_by_cols(p.cols, [&](auto shape) {
             constexpr int W = decltype(shape)::warps, J = decltype(shape)::quads;

@@ -161,7 +161,8 @@ def test_token_logprobs(ctx, R, V, pad, offset, k, T):
     check_logprobs(ctx, x, stride, k, T, tokens)
 
 
-@pytest.mark.parametrize("R,V,k,T", [(12, 600, 128, 1.0), (9, 5000, 20, 0.5), (8, 32001, 64, 1.0), (8, 32000, 128, 2.0), (8, 70000, 5, 1.0), (200, 9000, 33, 1.0)])
+@pytest.mark.parametrize("R,V,k,T", [(12, 600, 128, 1.0), (9, 5000, 20, 0.5), (8, 32001, 64, 1.0), (8, 32000, 128, 2.0), (8, 70000, 5, 1.0), (200, 9000, 33, 1.0), (150, 4097, 50, 1.0),
+                                     (20, 16384, 128, 0.7), (21, 16385, 128, 1.0), (900, 9000, 20, 1.0), (500, 3001, 64, 1.0)])
 @pytest.mark.parametrize("rounded", [False, True])
 def test_token_logprobs_of_masked_and_extreme_rows(ctx, R, V, k, T, rounded):
     x, stride = make_logits(R, V, 1, 1, seed=2, rounded=rounded)
@@ -251,7 +252,7 @@ def test_top_tokens_of_many_equal_values(ctx):
         check_logprobs(ctx, x, V, min(V, 100), 1.0, torch.zeros(40, dtype=torch.long))
 
 
-@pytest.mark.parametrize("R,V", [(6, 300), (6, 32000)])
+@pytest.mark.parametrize("R,V", [(6, 300), (6, 32000), (6, 5000), (6, 16000)])
 def test_rows_with_nan_or_infinity(ctx, R, V):
     x, stride = make_logits(R, V, seed=3)
     x[1, V // 3] = math.nan
