@@ -4,7 +4,7 @@
 // Bound by memory: a forward call reads the logits once, a gradient reads them and writes as much; next to that the issue slots, of which an fp32 value takes
 // 11.8 thread-instructions where only its statistics are wanted (pairs of values an instruction) and 20.5 with the 20 largest sought.
 // 4096 x 32000 (524 MB; a copy would take 81.5 us for its bytes, 163 us for read and written): log probabilities and entropy 78 us, with the 20 most probable
-// tokens 110 us, their gradient 161 us; distillation from lists of 64: loss 80 us, loss and gradient in one call 191 us, gradient from kept statistics 176 us.
+// tokens 110 us, their gradient 161 us; distillation from lists of 64: loss 80 us, loss and gradient in one call 184 us, gradient from kept statistics 176 us.
 //
 // With T the temperature, m the largest logit of a row and d_c = (x_c - m) / T:
 //     s = sum exp(d_c)      log p_c = d_c - ln s      H = ln s - (sum exp(d_c) d_c) / s
@@ -1532,23 +1532,30 @@ int row_cluster(const VocabRows& p, int sm_count) {
     while (n < kMaxCluster && ((p.rows * 2 * n <= 2 * (size_t)sm_count && p.cols / (2 * n) >= 2048) || (p.rows * 2 * n <= most * sm_count && p.cols / (2 * n) >= least))) n *= 2;
     return n;
 }
-// f(warps of a row, quads of a lane) by the columns
-template <int W, int J>
-struct Short { static constexpr int warps = W, quads = J; };
-template <class F>
-cudaError_t short_by_cols(int cols, F f) {
-    if (cols <= 512) return f(Short<1, 4>());
-    if (cols <= 1024) return f(Short<1, 8>());
-    if (cols <= 2048) return f(Short<1, 16>());
-    if (cols <= 4096) return f(Short<2, 16>());
-    return cols <= 8192 ? f(Short<4, 16>()) : f(Short<8, 16>());
-}
 // Up to how many columns.  11000 x 8192 by CTAs / by warps: statistics 60 / 77 us, lists' loss 80 / 82, the gradient of log probabilities 111 / 111, of lists 116 / 111, loss
 // and gradient 225 / 128; 3000 x 16384 of these 77 in the ring / 75.  Fewer rows than three an SM: 300 x 2000 statistics 3.7 / 3.3 us, their gradient 3.3 / 3.9.
 // With tokens sought: 600 x 2000 with 20 / 64 of them 9.1 / 9.0 us and 13 / 17 (four rows an SM), 11000 x 2000 99 / 46 and 143 / 81, 3000 x 1000 28 / 10 and 41 / 16.  Below 1024
 // columns a CTA has warps without values, which leave it no bound: 1 x 500 18 / 5.5 us, 11000 x 500 769 / 19; 1 x 1024 4.5 / 6.3.  Statistics alone, which are
 // the same bits then: 20 x 1000 2.6 / 2.6.
 constexpr int kShortAll = 1023, kShortTop = 2048, kShortStats = 4096, kShortGrad = 4096, kShortListGrad = 8192, kShortBoth = 16384;
+// f(warps of a row, quads of a lane) by the columns, MOST at most
+template <int W, int J>
+struct Short { static constexpr int warps = W, quads = J; };
+template <int MOST, class F>
+cudaError_t short_by_cols(int cols, F f) {
+    if (cols <= 512) return f(Short<1, 4>());
+    if (cols <= 1024) return f(Short<1, 8>());
+    if constexpr (MOST > 4096) {
+        if (cols > 8192) {
+            if constexpr (MOST > 8192) return f(Short<8, 16>());
+        }
+        if (cols > 4096) return f(Short<4, 16>());
+    }
+    if constexpr (MOST > 2048) {
+        if (cols > 2048) return f(Short<2, 16>());
+    }
+    return f(Short<1, 16>());
+}
 bool short_rows(size_t rows, int cols, int most, int sm_count) { return cols <= most && rows >= 3 * (size_t)sm_count; }
 bool short_forward(const VocabRows& p, int sm_count) {
     if (p.n_teacher == 0 && p.cols <= kShortAll) return true;
@@ -1574,15 +1581,19 @@ cudaError_t launch_held_tops(const VocabRows& p, int sm_count, cudaStream_t stre
 }
 cudaError_t launch_forward(VocabRows& p, int sm_count, cudaStream_t stream) {
     if (held_tops(p, sm_count)) return launch_held_tops(p, sm_count, stream);
-    if (short_forward(p, sm_count))
-        return short_by_cols(p.cols, [&](auto shape) {
-            constexpr int W = decltype(shape)::warps, J = decltype(shape)::quads;
-            if constexpr (W == 1)
-                if (p.n_top) return launch_rows(p.entropy ? short_rows_kernel<W, J, true, kTop> : short_rows_kernel<W, J, false, kTop>, short_grid(p.rows, W, sm_count), kRowThreads, 1, 0, stream, p);
-            const auto kern = p.n_teacher ? (p.grad_logits ? short_rows_kernel<W, J, false, kGrad> : short_rows_kernel<W, J, false, kList>)
-                                          : p.entropy ? short_rows_kernel<W, J, true, kPlain> : short_rows_kernel<W, J, false, kPlain>;
-            return launch_rows(kern, short_grid(p.rows, W, sm_count), kRowThreads, 1, 0, stream, p);
+    if (short_forward(p, sm_count)) {
+        const auto launch = [&](auto kern, int warps) { return launch_rows(kern, short_grid(p.rows, warps, sm_count), kRowThreads, 1, 0, stream, p); };
+        if (p.grad_logits)
+            return short_by_cols<kShortBoth>(p.cols, [&](auto w) { return launch(short_rows_kernel<decltype(w)::warps, decltype(w)::quads, false, kGrad>, w.warps); });
+        if (p.n_top)
+            return short_by_cols<kShortTop>(p.cols, [&](auto w) {
+                return p.entropy ? launch(short_rows_kernel<1, decltype(w)::quads, true, kTop>, 1) : launch(short_rows_kernel<1, decltype(w)::quads, false, kTop>, 1);
+            });
+        return short_by_cols<kShortStats>(p.cols, [&](auto w) {
+            constexpr int W = decltype(w)::warps, J = decltype(w)::quads;
+            return p.n_teacher ? launch(short_rows_kernel<W, J, false, kList>, W) : p.entropy ? launch(short_rows_kernel<W, J, true, kPlain>, W) : launch(short_rows_kernel<W, J, false, kPlain>, W);
         });
+    }
     p.cluster = row_cluster(p, sm_count);
     // Bounds after 1, 2, 4, 8, ... steps, between two of which there are as many hits again; after 1 and 2 only where a barrier and a bound are more than the
     // hits they save.  All of them / two, k = 20: 4096 x 32000 (8 steps) 112 / 110 us, 2000 x 50003 82 / 86, 600 x 128256 69 / 122; k = 64:
@@ -1650,11 +1661,11 @@ void temperature_of(float t, float* c, float* inv_t) {
     *c = (float)(1.4426950408889634 / (double)t);
 }
 cudaError_t launch_grad(bool distill, VocabGrad& p, int sm_count, cudaStream_t stream) {
-    if (short_rows(p.rows, p.cols, distill ? kShortListGrad : kShortGrad, sm_count))
-        return short_by_cols(p.cols, [&](auto shape) {
-            constexpr int W = decltype(shape)::warps, J = decltype(shape)::quads;
-            return launch_rows(distill ? short_grad_kernel<W, J, true> : short_grad_kernel<W, J, false>, short_grid(p.rows, W, sm_count), kRowThreads, 1, 0, stream, p);
-        });
+    if (short_rows(p.rows, p.cols, distill ? kShortListGrad : kShortGrad, sm_count)) {
+        const auto launch = [&](auto kern, int warps) { return launch_rows(kern, short_grid(p.rows, warps, sm_count), kRowThreads, 1, 0, stream, p); };
+        return distill ? short_by_cols<kShortListGrad>(p.cols, [&](auto w) { return launch(short_grad_kernel<decltype(w)::warps, decltype(w)::quads, true>, w.warps); })
+                       : short_by_cols<kShortGrad>(p.cols, [&](auto w) { return launch(short_grad_kernel<decltype(w)::warps, decltype(w)::quads, false>, w.warps); });
+    }
     // tiles of a row where the rows are fewer than the CTAs that fill the SMs
     const size_t want = 4 * (size_t)sm_count;
     p.tiles = 1;
