@@ -1168,9 +1168,10 @@ __global__ void __launch_bounds__(kRowThreads, 4) vocab_grad_kernel(VocabGrad p)
         else write_part<kRowThreads>(part, q, g, v, loose, terms.none, with_entropy);
         __syncthreads();
         if (!DISTILL && threadIdx.x == 0 && !terms.none && terms.token >= c0 && terms.token < c0 + cn) g[terms.token - c0] = with_entropy(x_token) + terms.up;
-        if (DISTILL && warp == 0 && !terms.none) {
-            copies_wait<0>();
+        if (DISTILL && warp == 0) {
+            copies_wait<0>();                                     // whatever the row asks for: the next item's list comes to the same place
             __syncwarp();
+            if (terms.none) continue;
             for (int i = lane; i < p.n_teacher; i += 32)
                 if (list.id[i] < 0 || list.id[i] >= p.cols) list.t[i] = -INFINITY;
             list_terms(list, p);

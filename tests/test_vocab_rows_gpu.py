@@ -534,6 +534,27 @@ def test_distillation_lists_and_rows_that_go_wrong(ctx, R, V, form):
     assert float(part[0]) == math.inf and float(part[11]) == 0.0
 
 
+@pytest.mark.parametrize("form", ["split", "split in place"])
+def test_lists_of_a_ctas_next_rows(ctx, form):
+    """Three rows a CTA of the gradient's kernel, whose lists come to the same place: behind rows of which nothing is asked, behind rows with a list of
+    their own, and none behind a list."""
+    V, K, per = 8300, 20, 16 * ctx.sm_count
+    R = 2 * per + 300
+    x, stride = make_logits(R, V, 0, 0, seed=41)
+    ids, a = make_teacher(R, V, K, 9)
+    ids[:400] = -1
+    ids[300:400, 7] = V
+    x[600:700] = NEG
+    ids[per + 200:per + 400] = -1
+    ids[per + 700:per + 800, 1:] = -1
+    ids[2 * per + 100:2 * per + 150] = -1
+    rows = torch.cat([torch.arange(900), torch.arange(per, per + 900), torch.arange(2 * per, R)])
+    losses, tol_l, grad, tol_g = distill_ref(x[rows.to(x.device)], ids[rows], a[rows], 2.0, 1.5 * len(rows) / R)
+    part, out, got = run_distill(ctx, x, stride, ids, a, 2.0, 1.5, form)
+    near(part[rows], losses, tol_l, "losses")
+    near(got[rows], grad, tol_g, "gradient")
+
+
 @pytest.mark.parametrize("form", FORMS)
 @pytest.mark.parametrize("K", [33, 64, 128])
 def test_distillation_lists_longer_than_a_warp(ctx, K, form):
