@@ -1057,9 +1057,11 @@ __global__ void __launch_bounds__(kRingThreads + 64, 1) distill_ring_kernel(Voca
         }
         // an empty list or an empty row has no gradient; a list that is not a number has none that is one
         const TeacherList& list = list_warp.of(item);
-        const float m = st.m, s = st.s, sg = gradient_sum(s, list.sum), f = sg == 0.0f ? 0.0f : up / sg;
+        const float m = st.m, s = st.s, sg = gradient_sum(s, list.sum);
+        const bool none = sg == 0.0f;
+        const float f = none ? 0.0f : up / sg;                    // 0 too where it underflows: the listed tokens' gradients may not
         if (of_lists) {
-            if (!(sg == 0.0f)) list_gradients(list_warp.of(item), p.n_teacher, up, ProbGrad{m, p.c, f});
+            if (!none) list_gradients(list_warp.of(item), p.n_teacher, up, ProbGrad{m, p.c, f});
             __syncwarp();
             if (lane == 0)
                 for (int c = 0; c < r.chunks; ++c) {
@@ -1072,15 +1074,15 @@ __global__ void __launch_bounds__(kRingThreads + 64, 1) distill_ring_kernel(Voca
             list_warp.ahead(item);
             continue;
         }
-        if (threadIdx.x == 0) stat_none[item & 3] = f == 0.0f;
+        if (threadIdx.x == 0) stat_none[item & 3] = none;
         const ProbGrad value = {m, p.c, f};
-        if (has_loose) p.grad_logits[row * p.stride + c0 + part.loose(threadIdx.x)] = f == 0.0f ? 0.0f : value(loose);
+        if (has_loose) p.grad_logits[row * p.stride + c0 + part.loose(threadIdx.x)] = none ? 0.0f : value(loose);
 #pragma unroll 1
         for (int c = 0; c < r.chunks; ++c) {
             const int n = min(r.chunk, part.n4 - c * r.chunk);
             float4* chunk = ring + slot * r.chunk;
 #pragma unroll 4
-            for (int i = threadIdx.x; i < n; i += kRingThreads) chunk[i] = f == 0.0f ? make_float4(0.f, 0.f, 0.f, 0.f) : quad_of(chunk[i], value);
+            for (int i = threadIdx.x; i < n; i += kRingThreads) chunk[i] = none ? make_float4(0.f, 0.f, 0.f, 0.f) : quad_of(chunk[i], value);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&done[slot])) : "memory");

@@ -599,6 +599,18 @@ def test_distillation_of_rows_with_nan(ctx, R, V, form):
     assert float(part[2]) == 0.0 and bool((got[2] == 0.0).all())
 
 
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("R,V,pad", [(8, 3000, 0), (512, 900, 0), (512, 17000, 0), (512, 6001, 1), (256, 30000, 0)])
+def test_gradients_of_listed_tokens_beside_probabilities_that_underflow(ctx, R, V, pad, form):
+    up = 2.0 ** -147
+    x, stride = make_logits(R, V, pad, 0, seed=42)
+    x.zero_()
+    ids = torch.arange(R, dtype=torch.int32)[:, None] * 3 % V
+    part, out, got = run_distill(ctx, x, stride, ids, torch.zeros(R, 1), 1.0, R * up, form)
+    want = torch.zeros(R, V).scatter_(1, ids.long(), -up)
+    assert torch.equal(got.cpu(), want)
+
+
 def test_a_teachers_list_and_its_log_probabilities_teach_the_same(ctx):
     """What token_logprobs keeps of a teacher, put into distillation_loss: the same loss as from its logits, and 0 for a student that
     gives these tokens alone its probability."""
