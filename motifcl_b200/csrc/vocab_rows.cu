@@ -842,7 +842,7 @@ __global__ void __launch_bounds__(kRowThreads, 4) vocab_rows_kernel(VocabRows p)
             const float sg = gradient_sum(s, list_warp.of(item).sum);
             gm = m;
             gf = up / sg;
-            none = sg == 0.0f;
+            none = sg == 0.0f || up == 0.0f;
         }
         if (of_lists) {
             const TeacherList& list = list_warp.of(item);
@@ -1055,10 +1055,10 @@ __global__ void __launch_bounds__(kRingThreads + 64, 1) distill_ring_kernel(Voca
             st.m = __shfl_sync(0xffffffffu, st.m, 0);
             st.s = __shfl_sync(0xffffffffu, st.s, 0);
         }
-        // an empty list or an empty row has no gradient; a list that is not a number has none that is one
+        // an empty list or an empty row has no gradient, nor has a loss of which none is asked; a list that is not a number has none that is one
         const TeacherList& list = list_warp.of(item);
         const float m = st.m, s = st.s, sg = gradient_sum(s, list.sum);
-        const bool none = sg == 0.0f;
+        const bool none = sg == 0.0f || up == 0.0f;
         const float f = none ? 0.0f : up / sg;                    // 0 too where it underflows: the listed tokens' gradients may not
         if (of_lists) {
             if (!none) list_gradients(list_warp.of(item), p.n_teacher, up, ProbGrad{m, p.c, f});
@@ -1121,6 +1121,7 @@ __device__ __forceinline__ Terms grad_terms(const VocabGrad& p, size_t row, floa
     Terms t = {0.0f, 0.0f, 0.0f, -1, s == 0.0f};
     if (DISTILL) {
         t.up = load_behind(p.grad_out) * p.inv_t / (float)p.rows;
+        t.none = t.none || t.up == 0.0f;
         t.k0 = t.up / s;
         return t;
     }
@@ -1412,10 +1413,11 @@ __global__ void __launch_bounds__(kRowThreads) short_rows_kernel(VocabRows p) {
         if (DISTILL && lead) list_result(p, list, row, m, s, list_loss(list, p.n_teacher, log_prob));
         if (GRAD) {
             const float sg = gradient_sum(s, list.sum);
+            const bool none = sg == 0.0f || up == 0.0f;
             const ProbGrad value = {m, p.c, up / sg};
-            r.write(p.grad_logits + row * p.stride, sg == 0.0f, value);
+            r.write(p.grad_logits + row * p.stride, none, value);
             row_sync<W>();
-            if (lead && !(sg == 0.0f)) list_write(list, p.n_teacher, p.grad_logits + row * p.stride, 0, p.cols, up, value);
+            if (lead && !none) list_write(list, p.n_teacher, p.grad_logits + row * p.stride, 0, p.cols, up, value);
         }
         if (DISTILL) __syncwarp();                                // before the next row's list comes
     }

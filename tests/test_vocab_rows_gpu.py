@@ -600,6 +600,17 @@ def test_distillation_of_rows_with_nan(ctx, R, V, form):
 
 
 @pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("R,V,pad", [(7, 3000, 0), (300, 25001, 1), (160, 60001, 0), (460, 900, 0), (460, 2500, 1), (450, 8000, 0), (450, 12001, 0), (460, 18000, 0)])
+def test_gradient_is_exactly_zero_where_the_losss_gradient_is(ctx, R, V, pad, form):
+    x, stride = make_logits(R, V, pad, 0, seed=43)
+    ids, a = make_teacher(R, V, 5, 10)
+    x[0, 7], x[1, V - 1], x[2], x[3] = math.nan, math.inf, math.nan, NEG
+    a[4, 2], a[5, 2] = math.nan, math.inf
+    part, out, got = run_distill(ctx, x, stride, ids, a, 1.0, 0.0, form)
+    assert bool((got == 0.0).all())
+
+
+@pytest.mark.parametrize("form", FORMS)
 @pytest.mark.parametrize("R,V,pad", [(8, 3000, 0), (512, 900, 0), (512, 17000, 0), (512, 6001, 1), (256, 30000, 0)])
 def test_gradients_of_listed_tokens_beside_probabilities_that_underflow(ctx, R, V, pad, form):
     up = 2.0 ** -147
