@@ -369,7 +369,7 @@ int mcl_cuda_layernorm_backward(mcl_cuda_ctx* ctx, const float* x, const float* 
  *                             pass over the logits.  No factor temperature^2 is applied.
  *   ..._backward              the same gradient from row_stats, for a grad_out that is known later.  These row_stats are distillation_loss's own: s is 0
  *                             in a row without entries, and not a number where the list is none
- * grad_logits has the logits' stride, may be the logits themselves but overlap them in no other way, and is exactly 0 in rows that nothing asks anything of (a token or ids
+ * grad_logits has the logits' stride, may be the logits themselves but overlap them in no other way (its rows may lie between theirs), and is exactly 0 in rows that nothing asks anything of (a token or ids
  * outside the vocabulary and no other gradient, or gradients of 0), whatever these rows hold.
  * Logits of -infinity (or the lowest float) are masked: p = 0, no part in the entropy, gradient 0.  A row of nothing but -infinity has
  * logprobs and top_logprobs -infinity, entropy 0, an infinite distillation loss (0 without entries) and gradient 0.  A row with a NaN or +infinity gives NaN, and ids

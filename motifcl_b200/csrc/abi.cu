@@ -1431,13 +1431,16 @@ int check_vocab(mcl_cuda_ctx* ctx, const char* op, const float* logits, size_t r
         return fail(ctx, MCL_CUDA_EINVAL, std::string(op) + " requires a temperature from 1e-30 to 1e30");
     return check_ptr(ctx, op, "logits", logits, 4);
 }
-// grad_logits may be the logits themselves, and overlap them in no other way
+// grad_logits may be the logits themselves, and overlap them in no other way; rows of one between those of the other do not overlap
 int check_grad_logits(mcl_cuda_ctx* ctx, const char* op, const float* logits, const float* grad_logits, size_t rows, size_t cols, size_t row_stride) {
     MCL_TRY(check_ptr(ctx, op, "grad_logits", grad_logits, 4));
     const uintptr_t a = reinterpret_cast<uintptr_t>(logits), b = reinterpret_cast<uintptr_t>(grad_logits);
     const size_t span = ((rows - 1) * row_stride + cols) * sizeof(float);
-    if (a != b && a < b + span && b < a + span)
-        return fail(ctx, MCL_CUDA_EINVAL, std::string(op) + ": grad_logits overlaps logits without being the same");
+    if (a != b && a < b + span && b < a + span) {
+        const size_t row = row_stride * sizeof(float), used = cols * sizeof(float), behind = (a < b ? b - a : a - b) % row;
+        if (behind < used || behind > row - used)
+            return fail(ctx, MCL_CUDA_EINVAL, std::string(op) + ": grad_logits overlaps logits without being the same");
+    }
     return MCL_CUDA_OK;
 }
 int check_teacher(mcl_cuda_ctx* ctx, const char* op, const int32_t* teacher_ids, const float* teacher_logits, size_t n_teacher) {

@@ -645,6 +645,28 @@ def test_a_teachers_list_and_its_log_probabilities_teach_the_same(ctx):
     near(same[2], grad, tol_g)
 
 
+@pytest.mark.parametrize("R,V", [(1, 300), (7, 3000), (300, 25000), (460, 901), (460, 9000)])
+@pytest.mark.parametrize("first", [False, True])
+def test_logits_and_gradients_side_by_side(ctx, R, V, first):
+    stride = 2 * V + 8
+    x0, _ = make_logits(R, V, seed=44)
+    ids, a = make_teacher(R, V, 5, 11)
+    losses, tol_l, grad, tol_g = distill_ref(x0, ids, a, 1.0, 1.0)
+    for form in range(2):
+        both = torch.full((R, stride), 5.0, device="cuda")
+        x, got = (both[:, V + 4:2 * V + 4], both[:, :V]) if first else (both[:, :V], both[:, V + 4:2 * V + 4])
+        x.copy_(x0)
+        one, part, out, stats = torch.ones(1, device="cuda"), torch.empty(R, device="cuda"), torch.empty(1, device="cuda"), torch.empty(R, 2, device="cuda")
+        if form == 0:
+            ctx.distillation_loss(x, ids.cuda(), a.cuda(), part, out, stats, one, got, R, V, 5, 1.0, stride)
+        else:
+            ctx.distillation_loss(x, ids.cuda(), a.cuda(), part, out, stats, None, None, R, V, 5, 1.0, stride)
+            ctx.distillation_loss_backward(x, ids.cuda(), a.cuda(), stats, one, got, R, V, 5, 1.0, stride)
+        torch.cuda.synchronize()
+        near(got, grad, tol_g)
+        assert torch.equal(x, x0) and bool((both[:, V:V + 4] == 5.0).all()) and bool((both[:, 2 * V + 4:] == 5.0).all())
+
+
 # ---- streams, recordings, repetition --------------------------------------------------------------------------------------
 
 def test_recorded_and_replayed_with_new_inputs(ctx):
