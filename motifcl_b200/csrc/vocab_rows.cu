@@ -483,6 +483,7 @@ struct VocabRows {
     int n_teacher;
     float* losses;
     const float* grad_out;             // with grad_logits
+    float per_row;                     // 1 / (T rows)
     float* grad_logits;
     int* err_word;                     // where a bounded wait gives up
 };
@@ -688,7 +689,7 @@ __global__ void __launch_bounds__(kRowThreads, 4) vocab_rows_kernel(VocabRows p)
     if (of_lists) list_warp.start();
     Stream<THREADS, decltype(part_of)> stream(dynamic, part_of, of_lists ? 0 : mine, cn);
     const int q = stream.q;
-    const float up = GRAD ? load_behind(p.grad_out) * p.inv_t / (float)p.rows : 0.0f;
+    const float up = GRAD ? load_behind(p.grad_out) * p.per_row : 0.0f;
     // GRAD, of the row before too, whose listed tokens are written when all of its gradient is
     float gm = 0.0f, gf = 0.0f;
     bool none = true;
@@ -924,7 +925,7 @@ __global__ void __launch_bounds__(kRingThreads + 64, 1) distill_ring_kernel(Voca
     auto row_of = [&](size_t i) { return first + i * step; };
     auto part_of = [&](size_t i) { return Part(p.logits + row_of(i) * p.stride + c0, cn); };
     ListWarp<kRingLists, VocabRows, decltype(row_of)> list_warp = {lists, p, mine, row_of};
-    const float up = load_behind(p.grad_out) * p.inv_t / (float)p.rows;
+    const float up = load_behind(p.grad_out) * p.per_row;
     // Where a wait runs out the call's results are void: the error word says so, nobody waits any more, and every loop runs to its end.
     auto gone = [&] {
         if (lane == 0) {
@@ -1107,6 +1108,7 @@ struct VocabGrad {
     const float* teacher_logits;
     int n_teacher;
     const float* grad_out;
+    float per_row;                     // 1 / (T rows)
     float* grad_logits;
 };
 
@@ -1120,7 +1122,7 @@ template <bool DISTILL>
 __device__ __forceinline__ Terms grad_terms(const VocabGrad& p, size_t row, float m, float s) {
     Terms t = {0.0f, 0.0f, 0.0f, -1, s == 0.0f};
     if (DISTILL) {
-        t.up = load_behind(p.grad_out) * p.inv_t / (float)p.rows;
+        t.up = load_behind(p.grad_out) * p.per_row;
         t.none = t.none || t.up == 0.0f;
         t.k0 = t.up / s;
         return t;
@@ -1371,7 +1373,7 @@ __global__ void __launch_bounds__(kRowThreads) short_rows_kernel(VocabRows p) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const bool lead = warp % W == 0;   // the warp that has the row's list and results
     TeacherList& list = lists[DISTILL ? warp / W : 0];
-    const float up = GRAD ? load_behind(p.grad_out) * p.inv_t / (float)p.rows : 0.0f;
+    const float up = GRAD ? load_behind(p.grad_out) * p.per_row : 0.0f;
     int turn = 0;
     for (size_t row = (size_t)blockIdx.x * G + warp / W; row < p.rows; row += (size_t)gridDim.x * G) {
         const float* x = p.logits + row * p.stride;
@@ -1665,6 +1667,8 @@ void temperature_of(float t, float* c, float* inv_t) {
     *inv_t = 1.0f / t;
     *c = (float)(1.4426950408889634 / (double)t);
 }
+// One factor, so that no product on the way leaves fp32 where the result does not.
+float per_row_of(float t, size_t rows) { return (float)(1.0 / ((double)t * (double)rows)); }
 cudaError_t launch_grad(bool distill, VocabGrad& p, int sm_count, cudaStream_t stream) {
     if (short_rows(p.rows, p.cols, distill ? kShortListGrad : kShortGrad, sm_count)) {
         const auto launch = [&](auto kern, int warps) { return launch_rows(kern, short_grid(p.rows, warps, sm_count), kRowThreads, 1, 0, stream, p); };
@@ -1709,7 +1713,7 @@ cudaError_t launch_distillation_loss(const float* logits, const int* teacher_ids
     p.logits = logits; p.rows = rows; p.stride = stride; p.cols = cols;
     temperature_of(temperature, &p.c, &p.inv_t);
     p.teacher_ids = teacher_ids; p.teacher_logits = teacher_logits; p.n_teacher = n_teacher;
-    p.losses = losses; p.row_stats = row_stats; p.grad_out = grad_out; p.grad_logits = grad_logits;
+    p.losses = losses; p.row_stats = row_stats; p.grad_out = grad_out; p.per_row = per_row_of(temperature, rows); p.grad_logits = grad_logits;
     p.err_word = err_word;
     const cudaError_t e = grad_logits != nullptr && ring_takes(p, sm_count, max_smem) ? launch_ring(p, sm_count, stream) : launch_forward(p, sm_count, stream);
     return e != cudaSuccess ? e : launch_mean(losses, out, rows, rows, stream);
@@ -1721,7 +1725,7 @@ cudaError_t launch_distillation_loss_backward(const float* logits, const int* te
     p.logits = logits; p.rows = rows; p.stride = stride; p.cols = cols;
     temperature_of(temperature, &p.c, &p.inv_t);
     p.teacher_ids = teacher_ids; p.teacher_logits = teacher_logits; p.n_teacher = n_teacher; p.row_stats = row_stats;
-    p.grad_out = grad_out; p.grad_logits = grad_logits;
+    p.grad_out = grad_out; p.per_row = per_row_of(temperature, rows); p.grad_logits = grad_logits;
     return launch_grad(true, p, sm_count, stream);
 }
 }  // namespace mcl

@@ -645,6 +645,16 @@ def test_a_teachers_list_and_its_log_probabilities_teach_the_same(ctx):
     near(same[2], grad, tol_g)
 
 
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("R,V,pad", [(8, 3000, 0), (512, 900, 0), (512, 17000, 0), (512, 6001, 1)])
+def test_gradient_of_the_smallest_temperature(ctx, R, V, pad, form):
+    x, stride = make_logits(R, V, pad, 0, seed=45)
+    ids, a = make_teacher(R, V, 3, 12)
+    losses, tol_l, grad, tol_g = distill_ref(x, ids, a, 1e-30, 1e9)
+    part, out, got = run_distill(ctx, x, stride, ids, a, 1e-30, 1e9, form)
+    near(got, grad, tol_g)
+
+
 @pytest.mark.parametrize("R,V", [(1, 300), (7, 3000), (300, 25000), (460, 901), (460, 9000)])
 @pytest.mark.parametrize("first", [False, True])
 def test_logits_and_gradients_side_by_side(ctx, R, V, first):
