@@ -20,6 +20,23 @@ def _ptr(t):
     return t.data_ptr()
 
 
+# _ptr of a tensor whose elements have to be of one type: the C call gets an address alone and would read another type's bits as if they were these.
+def _f32(t):
+    if t is None or isinstance(t, int):
+        return t
+    if t.dtype.itemsize != 4 or not t.dtype.is_floating_point:
+        raise MotifclCudaError(1, f"a float32 tensor is needed, not {t.dtype}")
+    return t.data_ptr()
+
+
+def _ids(t):
+    if t is None or isinstance(t, int):
+        return t
+    if t.dtype.itemsize != 4 or t.dtype.is_floating_point:
+        raise MotifclCudaError(1, f"ids of tokens must be int32, not {t.dtype}")
+    return t.data_ptr()
+
+
 class LinearDesc(ctypes.Structure):
     """mcl_cuda_linear_desc: one layer of mcl_cuda_counter_linear_step_many."""
     _fields_ = [("x", ctypes.c_void_p), ("grad_out", ctypes.c_void_p), ("state", ctypes.c_void_p),
@@ -230,12 +247,12 @@ class Context:
 
     def layernorm(self, x, weight, bias, out, row_stats, rows, cols, eps):
         """bias and row_stats (mean and inverse deviation of each row, for the backward call) may be None."""
-        self._check(self._lib.mcl_cuda_layernorm(self._ctx, _ptr(x), _ptr(weight), _ptr(bias), _ptr(out), _ptr(row_stats), rows, cols, eps))
+        self._check(self._lib.mcl_cuda_layernorm(self._ctx, _f32(x), _f32(weight), _f32(bias), _f32(out), _f32(row_stats), rows, cols, eps))
 
     def layernorm_backward(self, x, weight, grad_out, row_stats, grad_x, grad_weight, grad_bias, rows, cols):
         """Any of the three gradients may be None."""
-        self._check(self._lib.mcl_cuda_layernorm_backward(self._ctx, _ptr(x), _ptr(weight), _ptr(grad_out), _ptr(row_stats), _ptr(grad_x),
-                                                          _ptr(grad_weight), _ptr(grad_bias), rows, cols))
+        self._check(self._lib.mcl_cuda_layernorm_backward(self._ctx, _f32(x), _f32(weight), _f32(grad_out), _f32(row_stats), _f32(grad_x),
+                                                          _f32(grad_weight), _f32(grad_bias), rows, cols))
 
     def mse_loss(self, pred, target, partial, out, n):
         """mean((pred - target)^2) with MotifCL's OpenCL summation order; partial: ceil(n / 256) floats."""
@@ -265,27 +282,27 @@ class Context:
                        row_stride=None):
         """ln p of each row's token, the row's entropy and its n_top most probable tokens; outputs that are None are not formed."""
         self._check(self._lib.mcl_cuda_token_logprobs(
-            self._ctx, _ptr(logits), _ptr(tokens), _ptr(logprobs), _ptr(entropy), _ptr(top_ids), _ptr(top_logprobs), _ptr(row_stats), rows, cols,
+            self._ctx, _f32(logits), _ids(tokens), _f32(logprobs), _f32(entropy), _ids(top_ids), _f32(top_logprobs), _f32(row_stats), rows, cols,
             cols if row_stride is None else row_stride, n_top, temperature))
 
     def token_logprobs_backward(self, logits, tokens, row_stats, entropy, grad_logprobs, grad_entropy, grad_logits, rows, cols, temperature=1.0,
                                 row_stride=None):
         """Gradient of the logits from those of logprobs and entropy (either may be None)."""
         self._check(self._lib.mcl_cuda_token_logprobs_backward(
-            self._ctx, _ptr(logits), _ptr(tokens), _ptr(row_stats), _ptr(entropy), _ptr(grad_logprobs), _ptr(grad_entropy), _ptr(grad_logits), rows,
+            self._ctx, _f32(logits), _ids(tokens), _f32(row_stats), _f32(entropy), _f32(grad_logprobs), _f32(grad_entropy), _f32(grad_logits), rows,
             cols, cols if row_stride is None else row_stride, temperature))
 
     def distillation_loss(self, logits, teacher_ids, teacher_logits, partial, out, row_stats, grad_out, grad_logits, rows, cols, n_teacher,
                           temperature=1.0, row_stride=None):
         """Loss against a teacher's kept tokens; with grad_out and grad_logits its gradient in the same pass."""
         self._check(self._lib.mcl_cuda_distillation_loss(
-            self._ctx, _ptr(logits), _ptr(teacher_ids), _ptr(teacher_logits), _ptr(partial), _ptr(out), _ptr(row_stats), _ptr(grad_out),
-            _ptr(grad_logits), rows, cols, cols if row_stride is None else row_stride, n_teacher, temperature))
+            self._ctx, _f32(logits), _ids(teacher_ids), _f32(teacher_logits), _f32(partial), _f32(out), _f32(row_stats), _f32(grad_out),
+            _f32(grad_logits), rows, cols, cols if row_stride is None else row_stride, n_teacher, temperature))
 
     def distillation_loss_backward(self, logits, teacher_ids, teacher_logits, row_stats, grad_out, grad_logits, rows, cols, n_teacher,
                                    temperature=1.0, row_stride=None):
         self._check(self._lib.mcl_cuda_distillation_loss_backward(
-            self._ctx, _ptr(logits), _ptr(teacher_ids), _ptr(teacher_logits), _ptr(row_stats), _ptr(grad_out), _ptr(grad_logits), rows, cols,
+            self._ctx, _f32(logits), _ids(teacher_ids), _f32(teacher_logits), _f32(row_stats), _f32(grad_out), _f32(grad_logits), rows, cols,
             cols if row_stride is None else row_stride, n_teacher, temperature))
 
     def token_position_embedding(self, token_weight, pos_weight, token_ids, out, token_count, vocab, seq_len, dim):
