@@ -357,6 +357,49 @@ def test_gradient_is_exactly_zero_where_nothing_is_asked(ctx):
     assert bool((grad[:4] == 0.0).all()) and bool((grad[4:] != 0.0).any())
 
 
+@pytest.mark.parametrize("R,V", [(460, 777), (450, 3001), (20, 20001)])
+def test_gradient_is_exactly_zero_where_nothing_is_asked_of_other_rows(ctx, R, V):
+    """Warps a row, and tiles of a row."""
+    x, stride = make_logits(R, V, 1, 0, seed=46)
+    x[0], x[1], x[2], x[3, V // 2] = math.nan, math.inf, NEG, math.nan
+    tokens = torch.full((R,), 4, dtype=torch.int32, device="cuda")
+    tokens[0], tokens[1] = -1, V + 5
+    dlogp, dent = torch.ones(R, device="cuda"), torch.zeros(R, device="cuda")
+    dlogp[3] = 0.0
+    fwd = run_logprobs(ctx, x, stride, tokens, 0, 1.0)
+    for second in (None, dent):
+        grad = torch.full((R * stride,), 3.0, device="cuda").view(R, stride)[:, :V]
+        ctx.token_logprobs_backward(x, tokens, fwd["stats"], fwd["H"] if second is not None else None, dlogp, second, grad, R, V, 1.0, stride)
+        torch.cuda.synchronize()
+        assert bool((grad[:4] == 0.0).all()) and bool((grad[4:] != 0.0).any(dim=1).all())
+
+
+@pytest.mark.parametrize("which", ["both", "logp"])
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("pad", [0, 1])
+def test_token_gradients_of_more_rows_than_ctas(ctx, which, in_place, pad):
+    """Three rows a CTA of the gradient's kernel."""
+    V, per = 4101, 16 * ctx.sm_count
+    R = 2 * per + 200
+    x, stride = make_logits(R, V, pad, 0, seed=47)
+    special_rows(x)
+    special_rows(x[per:])
+    special_rows(x[2 * per + 100:])
+    g = torch.Generator().manual_seed(48)
+    tokens = torch.randint(0, V, (R,), generator=g)
+    tokens[20:40], tokens[per + 30:per + 50], tokens[2 * per + 40:2 * per + 60] = -1, V, -1
+    dlogp, dent = torch.randn(R, generator=g), torch.randn(R, generator=g) if which == "both" else None
+    rows = torch.cat([torch.arange(200), torch.arange(per, per + 200), torch.arange(2 * per, R)])
+    want, tol = policy_grad(Row64(x[rows.to(x.device)], 1.0), tokens[rows], dlogp[rows], dent[rows] if dent is not None else None)
+    tokens = tokens.int().to("cuda")
+    fwd = run_logprobs(ctx, x, stride, tokens, 0, 1.0)
+    grad = x if in_place else torch.empty(R * stride, device="cuda").view(R, stride)[:, :V]
+    ctx.token_logprobs_backward(x, tokens, fwd["stats"], fwd["H"] if dent is not None else None, dlogp.to("cuda"), dent.to("cuda") if dent is not None else None, grad, R,
+                                V, 1.0, stride)
+    torch.cuda.synchronize()
+    near(grad[rows.to(grad.device)], want, tol)
+
+
 def test_gradients_against_differences(ctx):
     """Directional derivatives of the definitions in float64: differences of step h are off by h^2 / 6 of a third derivative (of order
     the value) and by 2^-52 / h: 1e-10 at h = 1e-5; the gradient itself by what policy_grad allows, below 1e-5 of its size here."""
@@ -532,6 +575,34 @@ def test_distillation_lists_and_rows_that_go_wrong(ctx, R, V, form):
     near(part, losses, tol_l, "losses")
     near(got, grad, tol_g, "gradient")
     assert float(part[0]) == math.inf and float(part[11]) == 0.0
+
+
+# (rows a wave, rows, columns, entries, pad, offset): rings of one CTA a row and of two, eight rows and more for each; the same rows with gradients that
+# start elsewhere between 16-byte boundaries, which go by a second time, three of them for each CTA
+@pytest.mark.parametrize("wave,R,V,K,pad,offset", [(148, 1300, 17000, 20, 0, 0), (148, 1250, 17003, 128, 1, 0), (74, 700, 50003, 7, 0, 0), (592, 1400, 17001, 20, 0, 1), (592, 1300, 17000, 64, 0, 2)])
+@pytest.mark.parametrize("form", ["one call", "in place"])
+def test_distillation_of_many_long_rows(ctx, wave, R, V, K, pad, offset, form):
+    x, stride = make_logits(R, V, pad, offset, seed=49)
+    ids, a = make_teacher(R, V, K, 13)
+    for first in range(0, R - wave, wave):                          # other rows than their neighbours' in every wave
+        turn = first // wave
+        special = torch.arange(first + 8 * turn, min(R, first + 8 * turn + 7))
+        if len(special) < 7:
+            continue
+        r = [int(i) for i in special]
+        ids[r[0]] = -1
+        ids[r[1], 1:] = -1
+        ids[r[2], 1:] = ids[r[2], 0]
+        ids[r[3], 0], ids[r[3], K - 1] = V - 1, 0
+        x[r[4]] = NEG
+        x[r[5], V // 3:] = NEG
+        a[r[6], 1:] = NEG
+    rows = torch.cat([torch.arange(min(100, wave)) + first for first in range(0, R, wave)] + [torch.arange(R - 20, R)])
+    rows = rows[rows < R].unique()
+    losses, tol_l, grad, tol_g = distill_ref(x[rows.to(x.device)], ids[rows], a[rows], 1.5, 0.75 * len(rows) / R)
+    part, out, got = run_distill(ctx, x, stride, ids, a, 1.5, 0.75, form)
+    near(part[rows.to(part.device)], losses, tol_l, "losses")
+    near(got[rows.to(got.device)], grad, tol_g, "gradient")
 
 
 @pytest.mark.parametrize("form", ["split", "split in place"])
