@@ -515,7 +515,7 @@ __device__ __forceinline__ void list_gather(TeacherList& l, const P& p, size_t r
         else l.t[i] = -INFINITY;
     }
 }
-// Probabilities t = exp2((a - top) c) / sum of the logits a.
+// Probabilities t = exp2((a - top) c) / sum of the logits a, and their logarithms, which only a loss needs.
 template <class P>
 __device__ __forceinline__ void list_terms(TeacherList& l, const P& p) {
     const int lane = threadIdx.x & 31;
@@ -1098,7 +1098,7 @@ struct VocabGrad {
     const float* logits;
     size_t rows, stride;
     int cols, tiles, per;              // tiles of a row, their length
-    float c, inv_t;
+    float c, inv_t;                    // of lists: 1 / (T rows)
     const float* row_stats;
     const int* tokens;
     const float* grad_logprobs;        // null: none
@@ -1108,7 +1108,6 @@ struct VocabGrad {
     const float* teacher_logits;
     int n_teacher;
     const float* grad_out;
-    float per_row;                     // 1 / (T rows)
     float* grad_logits;
 };
 
@@ -1122,7 +1121,7 @@ template <bool DISTILL>
 __device__ __forceinline__ Terms grad_terms(const VocabGrad& p, size_t row, float m, float s) {
     Terms t = {0.0f, 0.0f, 0.0f, -1, s == 0.0f};
     if (DISTILL) {
-        t.up = load_behind(p.grad_out) * p.per_row;
+        t.up = load_behind(p.grad_out) * p.inv_t;
         t.none = t.none || t.up == 0.0f;
         t.k0 = t.up / s;
         return t;
@@ -1725,7 +1724,7 @@ cudaError_t launch_distillation_loss_backward(const float* logits, const int* te
     p.logits = logits; p.rows = rows; p.stride = stride; p.cols = cols;
     temperature_of(temperature, &p.c, &p.inv_t);
     p.teacher_ids = teacher_ids; p.teacher_logits = teacher_logits; p.n_teacher = n_teacher; p.row_stats = row_stats;
-    p.grad_out = grad_out; p.per_row = per_row_of(temperature, rows); p.grad_logits = grad_logits;
+    p.grad_out = grad_out; p.inv_t = per_row_of(temperature, rows); p.grad_logits = grad_logits;
     return launch_grad(true, p, sm_count, stream);
 }
 }  // namespace mcl
