@@ -1529,11 +1529,12 @@ cudaError_t launch_rows(void (*kern)(P...), unsigned grid, int threads, int clus
 }
 // CTAs of a row: as many as leave none of the SMs idle, with 2048 logits each at least (one row of 32000: 6.8 us by eight, 16 rows 7.5).  Up to four on an SM (three
 // with a selection's shared memory) where a CTA's part stays long enough to pay for the cluster's seam.  One / two CTAs: 200 x 128256 statistics 23 / 20 us, with 20 tops
-// 33 / 26, lists' losses 27 / 22, but 150 x 50003 statistics 10.3 / 11.1; the gradient, a second pass over what L2 holds of a row, gains from shorter
+// 33 / 26, lists' losses 27 / 22, but 150 x 50003 statistics 10.3 / 11.1 (from 61440 on, where one CTA
+// takes a sixteenth step: 290 x 61400 14.8 / 16.9, 150 x 61400 11.1 / 11.8, 200 x 61500 14.5 / 13.3, 290 x 64000 16.1 / 15.0); the gradient, a second pass over what L2 holds of a row, gains from shorter
 // parts on: 150 x 24000 19 / 17.6, 200 x 14000 14.4 / 12.8.
 int row_cluster(const VocabRows& p, int sm_count) {
     const size_t most = p.n_top ? 3 : 4;
-    const int least = p.grad_logits ? 6144 : p.n_top || p.n_teacher ? 24576 : 30000;
+    const int least = p.grad_logits ? 6144 : p.n_top || p.n_teacher ? 24576 : 30720;
     int n = 1;
     while (n < kMaxCluster && ((p.rows * 2 * n <= 2 * (size_t)sm_count && p.cols / (2 * n) >= 2048) || (p.rows * 2 * n <= most * sm_count && p.cols / (2 * n) >= least))) n *= 2;
     return n;
