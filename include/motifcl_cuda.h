@@ -356,22 +356,24 @@ int mcl_cuda_layernorm_backward(mcl_cuda_ctx* ctx, const float* x, const float* 
  * asks for other outputs, or has other alignment, may round differently.
  *   token_logprobs            logprobs [rows] = ln p of the row's token (0 for a token outside [0, cols): padding; tokens and logprobs may be
  *                             NULL together); entropy [rows] (or NULL) = -sum p ln p; top_ids, top_logprobs [rows, n_top] (one of them may be
- *                             NULL, both with n_top = 0): the n_top largest logits' places and ln p, largest first, equal ones by their
- *                             place; row_stats [rows, 2] (or NULL) for the backward call: the largest logit m and s = sum exp((logit - m) /
+ *                             NULL, both with n_top = 0): the n_top largest logits' places and ln p (n_top is cols at most), largest first, equal ones by
+ *                             their place; row_stats [rows, 2] (or NULL) for the backward call: the largest logit m and s = sum exp((logit - m) /
  *                             temperature), so that the logarithm of the softmax's denominator is m / temperature + ln s
  *   ..._backward              grad_logits of sum(grad_logprobs . logprobs + grad_entropy . entropy); either gradient [rows] may be NULL (with it
  *                             tokens or entropy)
  *   distillation_loss         the Kullback-Leibler divergence of p from the teacher's kept tokens: t = softmax of the row's teacher_logits /
  *                             temperature over its entries, partial [rows] = sum t (ln t - ln p[id]), out[0] = their mean over all rows.
  *                             teacher_ids, teacher_logits [rows, n_teacher], logits or log probabilities (a constant per row falls out); an id
- *                             outside [0, cols) is no entry, a row without entries has loss 0; an id named twice is two entries.  With
+ *                             outside [0, cols), or a teacher_logit of -infinity, is no entry, a row without entries has loss 0; an id named twice is two entries.  With
  *                             grad_out and grad_logits (both or neither) also grad_logits = grad_out[0] * the gradient of out[0], in the same
  *                             pass over the logits.  No factor temperature^2 is applied.
  *   ..._backward              the same gradient from row_stats, for a grad_out that is known later.  These row_stats are distillation_loss's own: s is 0
  *                             in a row without entries, and not a number where the list is none
  * grad_logits has the logits' stride, may be the logits themselves but overlap them in no other way (its rows may lie between theirs), and is exactly 0 in rows that nothing asks anything of (a token or ids
  * outside the vocabulary and no other gradient, or gradients of 0), whatever these rows hold.
- * Logits of -infinity (or the lowest float) are masked: p = 0, no part in the entropy, gradient 0.  A row of nothing but -infinity has
+ * Logits of -infinity (or the lowest float) are masked: p = 0, no part in the entropy, gradient 0; but one that is the row's token or in its
+ * list keeps that token's own term, grad_logprobs / temperature or -grad_out[0] t / (temperature rows).  In a row with nothing above the lowest float that
+ * one is no mask.  exp((logit - m) / temperature) below 2^-126 is 0.  A row of nothing but -infinity has
  * logprobs and top_logprobs -infinity, entropy 0, an infinite distillation loss (0 without entries) and gradient 0.  A row with a NaN or +infinity gives NaN, and ids
  * of -1.  Lists have at most MCL_CUDA_LIST_MAX tokens. ---- */
 #define MCL_CUDA_LIST_MAX 128

@@ -218,7 +218,9 @@ __global__ void __launch_bounds__(256) rmsnorm_bwd_w_kernel(const float* x, cons
 // The variance is the mean of (x - mean)^2, not a difference of two sums, which a mean far from zero would leave no digits of.
 // Up to 8192 columns: W warps per row, each lane J times four columns in registers, the next row's loads in flight while this one's sums are formed, so
 // that memory sees every tensor once.  Bound by memory: 16384 x 2048 forward 44.6 us (6.0 TB/s), backward 66 us (6.1 TB/s); a CTA a row read again from L1, with a kernel of its
-// own for dw and db, 59 and 137; 4096 x 288 3.9 and 7.5 us (8.7 and 10.9), launches.  VEC: 16-byte accesses (rows on 16-byte boundaries); else a lane's columns are W * 32 apart, so that a warp's
+// own for dw and db, 59 and 137; 4096 x 288 3.9 and 7.5 us (8.7 and 10.9), launches.  Wider rows are further from it: 8192 x 4096 61 and 80 us
+// (4.4 and 5.0 TB/s), 4096 x 8192 76 and 89 us (3.5 and 4.5; backward one CTA of 1024 threads an SM, 48 bytes a thread not in its 64 registers), and scalar accesses cost the
+// backward pass more: 16384 x 2047 49 and 73 us, 8192 x 4095 51 and 116, 4096 x 8191 56 and 108.  VEC: 16-byte accesses (rows on 16-byte boundaries); else a lane's columns are W * 32 apart, so that a warp's
 // accesses are whole lines all the same.
 template <int W, int J, bool VEC>
 struct NormCols {
@@ -374,7 +376,8 @@ __global__ void __launch_bounds__(kNormThreads<W>) layernorm_bwd_rows_kernel(con
         }
     }
 }
-// Longer rows, which registers do not hold: a block per row, which is read again from L1; columns in blocks of 32 for dw and db.
+// Longer rows, which registers do not hold: a block per row, which is read again from L1; columns in blocks of 32 for dw and db, which read x and dy once more.
+// 2000 x 16384 forward 67 us (3.9 TB/s), backward 165 us; 2000 x 16383 128 and 195.
 __global__ void __launch_bounds__(256) layernorm_kernel(const float* x, const float* w, const float* b, float* out, float* row_stats, size_t rows,
                                                         Vec4 a, float eps) {
     grid_release();

@@ -3,13 +3,14 @@
 //
 // Bound by memory: a forward call reads the logits once, a gradient reads them and writes as much; next to that the issue slots, of which an fp32 value takes
 // 11.8 thread-instructions where only its statistics are wanted (pairs of values an instruction) and 20.5 with the 20 largest sought.
-// 4096 x 32000 (524 MB; a copy would take 81.5 us for its bytes, 163 us for read and written): log probabilities and entropy 78 us, with the 20 most probable
+// 4096 x 32000 (524 MB; at the rate of a copy its bytes take 81.5 us, 163 us read and written; a pass that only reads may be faster than that): log probabilities and entropy 78 us, with the 20 most probable
 // tokens 110 us, their gradient 161 us; distillation from lists of 64: loss 80 us, loss and gradient in one call 184 us, gradient from kept statistics 176 us.
 //
 // With T the temperature, m the largest logit of a row and d_c = (x_c - m) / T:
 //     s = sum exp(d_c)      log p_c = d_c - ln s      H = ln s - (sum exp(d_c) d_c) / s
 // so that both parts of H have one sign and nothing cancels.  m and s are kept apart (row_stats): their sum m / T + ln s would lose
-// the last digits of every log p_c where the logits are large.  Exponentials are 2^(d log2 e): one product, one ex2.approx, 2 ulp.
+// the last digits of every log p_c where the logits are large.  Exponentials are 2^(d log2 e): one product, one ex2.approx, 2 ulp; below 2^-126 they are 0.
+// log p_c takes (x_c - m) times the rounded 1 / T within the fma that takes ln s off: one rounding beside that of 1 / T, as many as a division would bring.
 // Masked logits (-infinity, the lowest float) and rows with nothing left fall out of one clamp: 2^-150 is 0 in fp32, and
 // 0 * -150 is 0 where 0 * -infinity is not a number.
 #include "kernels.h"
@@ -657,7 +658,7 @@ __device__ __forceinline__ void list_result(const VocabRows& p, const TeacherLis
 // TOP: a thread's first step is a sample of the row; the quads with something above the bound that it gives are noted as the row goes by, and
 // looked at again under the bound of all that the threads have seen.
 // That stays behind 1 % of the values of a long row and costs no second look at memory: 30 us of 110, which are issue slots (71 % of them
-// busy) and the barriers of a row.  Where more than kHits quads are noted (lists of 128 of long rows) the row is read again.
+// busy), the barriers of a row and 36 bytes a thread that 64 registers do not hold (lists: 8, with the gradient 204).  Where more than kHits quads are noted (lists of 128 of long rows) the row is read again.
 // LIST, GRAD: the last warp has the teacher's lists and forms the losses.  GRAD: the row goes by a second time (out of L2, where rows are few or short; long
 // ones go through the ring below), becomes its gradient, and that warp writes the listed tokens' gradients while the next row is at work.
 enum RowWork { kPlain, kTop, kList, kGrad };
